@@ -1,0 +1,480 @@
+// Attention of new tokens over their sequences' pages.
+//
+// Request i has T_i consecutive query tokens, the last of them at the last of its sequence's L_i keys: token t is at position L_i - T_i + t and
+// sees the keys at and before it, the nearest `window` of them if there is one.  The G query heads of a key-value head share its keys: they
+// and the tokens are the rows of one matrix product, row r = t * G + g.
+//
+// Structure: S^T = K Q^T and O^T += V^T P^T with v_mfma_f32_16x16x32_bf16.  A lane then holds the scores of ONE row (lane & 15) for four
+// consecutive keys a tile, the softmax's maximum and sum over keys are in-register steps and two lane exchanges, and the exponentials, packed
+// to bf16, are the second product's operand as they stand.  K fragments come straight from the pages (16 bytes a lane), V goes through LDS,
+// where ds_read_b64_tr_b16 hands out its transpose.  The softmax runs in one pass with a running maximum and sum in fp32 (base 2).
+//
+// Split: a workgroup takes a tile of rows of one request, one key-value head and one chunk of the keys; chunks are joined by a second launch.
+// Nothing about the lengths is known on the host, so every workgroup works out the split from them by itself (schedule()).
+#include "paged.h"
+
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+
+// ---------------------------------------------------------------------------------------------
+// The split.  Request i: R_i = G * T_i rows in rt_i tiles of TR, at most nb_i blocks of 64 keys a tile.  With W = sum rt_i * nb_i blocks of
+// work in all and `target` workgroups wanted, a chunk is at least S = max(min_blocks, W / target) blocks long and a tile of request i is cut
+// into C_i = clamp(floor(nb_i / S), 1, cmax) chunks of equal length: W / target + (number of tiles) items at most, whatever the lengths are,
+// and no item longer than 2 S.  Items are numbered request by request, tile by tile.
+// ---------------------------------------------------------------------------------------------
+struct Work { int req, seq, q0, T, L, tile, chunk, chunks; };
+
+static __device__ __forceinline__ void request_shape(const PagedAttnArgs& a, int i, int* seq, int* q0, int* T, int* L) {
+    *seq = a.seqs[i];
+    int c0 = a.cu[i], c1 = a.cu[i + 1];
+    c0 = min(max(c0, 0), a.n_tokens);
+    c1 = min(max(c1, c0), a.n_tokens);
+    *q0 = c0;
+    if ((unsigned)*seq < (unsigned)a.max_seqs) {
+        *T = c1 - c0;
+        *L = min(max(a.lens[*seq], 0), a.max_blocks << a.lps);
+    } else { *T = 0; *L = 0; }                              // padding: its rows are nobody's and stay as they are
+}
+template <int TR>
+static __device__ __forceinline__ void request_tiles(const PagedAttnArgs& a, int T, int L, int* rt, int* nb) {
+    *rt = (int)(((long)T * a.G + TR - 1) / TR);
+    int keys = L;
+    if (a.window) keys = (int)min((long)keys, (long)a.window + TR / a.G + 65);
+    *nb = (keys + 63) >> 6;
+}
+template <int NTH, int TR, class Want>
+static __device__ __forceinline__ bool schedule(const PagedAttnArgs& a, Want want, Work* out) {
+    __shared__ float fsum[NTH / 64];
+    __shared__ int isum[NTH / 64];
+    __shared__ Work found;
+    __shared__ int have;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (tid == 0) have = 0;
+    int seq, q0, T, L, rt = 0, nb = 0;
+    float w = 0.f;
+    for (int i0 = 0; i0 < a.n; i0 += NTH) {
+        if (i0 + tid < a.n) {
+            request_shape(a, i0 + tid, &seq, &q0, &T, &L);
+            request_tiles<TR>(a, T, L, &rt, &nb);
+            w += (float)rt * (float)nb;
+        }
+    }
+    w = wave_sum(w);
+    if (lane == 0) fsum[wave] = w;
+    __syncthreads();
+    float all = 0.f;
+#pragma unroll
+    for (int k = 0; k < NTH / 64; ++k) all += fsum[k];
+    const int S = max(a.min_blocks, (int)ceilf(fminf(all / (float)a.target, 1e9f)));
+    int base = 0;
+    for (int i0 = 0; i0 < a.n; i0 += NTH) {
+        int C = 1, items = 0;
+        if (a.n > NTH) {                                    // one request a thread: its numbers are still at hand
+            rt = nb = 0;
+            if (i0 + tid < a.n) { request_shape(a, i0 + tid, &seq, &q0, &T, &L); request_tiles<TR>(a, T, L, &rt, &nb); }
+        }
+        if (i0 + tid < a.n) { C = min(max(nb / S, 1), a.cmax); items = rt * C; }
+        int x = items;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) { const int y = __shfl_up(x, o, 64); if (lane >= o) x += y; }
+        if (lane == 63) isum[wave] = x;
+        __syncthreads();
+        int before = base;
+        for (int k = 0; k < NTH / 64; ++k) { if (k < wave) before += isum[k]; base += isum[k]; }
+        if (i0 + tid < a.n) {
+            Work f = {i0 + tid, seq, q0, T, L, 0, 0, C};
+            if (want(before + x - items, items, &f)) { found = f; have = 1; }
+        }
+        __syncthreads();
+        if (have) break;
+    }
+    if (!have) return false;
+    *out = found;
+    return true;
+}
+
+// the keys [lo, hi) that any row of tile `tile` sees, as blocks of 64 from lo rounded down; chunk c of C holds blocks [c * S, min(nb, (c+1) * S))
+struct Span { int lo, hi, first, nb, S; };
+static __device__ __forceinline__ Span tile_span(const PagedAttnArgs& a, const Work& w, int tile, int TR) {
+    Span s;
+    const int t0 = tile * TR / a.G, t1 = min((tile * TR + TR - 1) / a.G, w.T - 1);
+    s.hi = max(0, min(w.L, w.L - w.T + t1 + 1));
+    s.lo = a.window ? max(0, w.L - w.T + t0 + 1 - a.window) : 0;
+    s.first = s.lo & ~63;
+    s.nb = s.hi > s.lo ? (s.hi - s.first + 63) >> 6 : 0;
+    s.S = max(1, (s.nb + w.chunks - 1) / w.chunks);
+    return s;
+}
+
+static __device__ __forceinline__ bool nonfinite(bf16x8 v) {
+    const u32x4 u = __builtin_bit_cast(u32x4, v);
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bad |= (u[i] & 0x7f800000u) == 0x7f800000u || (u[i] & 0x7f80u) == 0x7f80u;
+    return bad;
+}
+static __device__ __forceinline__ bf16x8 e4m3x8(unsigned lo, unsigned hi) {        // exact: every e4m3 value is a bf16 value
+    bf16x8 r;
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true);
+    r[0] = a[0]; r[1] = a[1]; r[2] = b[0]; r[3] = b[1]; r[4] = c[0]; r[5] = c[1]; r[6] = d[0]; r[7] = d[1];
+    return r;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Few rows (a token, some drafted ones): bound by the bytes of K and V.  A workgroup's four waves take blocks of 32 keys in turn, each with a
+// softmax of its own and no barrier in the loop, and are merged at the end.  NT tiles of 16 rows share every K and V fragment.  The matrix
+// cores have time to spare, so P goes into the product as two bf16 halves (high and remainder): no precision is lost to its rounding.
+// ---------------------------------------------------------------------------------------------
+template <int D, bool E4M3, int NT>
+__global__ __launch_bounds__(256) void paged_attn_rows_kernel(PagedAttnArgs a) {
+    constexpr int KSQ = D / 32, DT = D / 16, VST = D + 16, TR = 16 * NT;
+    constexpr int NK = E4M3 ? KSQ / 2 : KSQ;               // 16-byte loads of one K tile a lane
+    constexpr int NV = E4M3 ? D / 32 : D / 16;             // 16-byte loads of 32 V rows a lane
+    constexpr int VCH = E4M3 ? D / 16 : D / 8;             // 16-byte chunks of a V row
+    __shared__ __attribute__((aligned(16))) bf16 Vs[4][32 * VST];
+    __shared__ float sm[4][16], sl[4][16];
+
+    const int item = blockIdx.x, hk = blockIdx.y;
+    Work w;
+    if (!schedule<256, TR>(a, [&](int first, int items, Work* f) {
+            const int k = item - first;
+            if (k < 0 || k >= items) return false;
+            f->tile = k / f->chunks; f->chunk = k - f->tile * f->chunks;
+            return true;
+        }, &w)) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int q4 = lane >> 4, r16 = lane & 15;
+    w.seq = __builtin_amdgcn_readfirstlane(w.seq); w.q0 = __builtin_amdgcn_readfirstlane(w.q0);
+    w.T = __builtin_amdgcn_readfirstlane(w.T); w.L = __builtin_amdgcn_readfirstlane(w.L);
+    w.tile = __builtin_amdgcn_readfirstlane(w.tile); w.chunk = __builtin_amdgcn_readfirstlane(w.chunk);
+    w.chunks = __builtin_amdgcn_readfirstlane(w.chunks);
+    const Span sp = tile_span(a, w, w.tile, TR);
+    const int b0 = w.chunk * sp.S, b1 = min(sp.nb, b0 + sp.S);
+    if (b0 >= b1 && w.chunk) return;                       // a chunk without keys; chunk 0 writes the zeros of rows that see nothing
+    const int R = w.T * a.G, base_pos = w.L - w.T;
+
+    // rows of this lane (one a tile) and their queries
+    int pos[NT];
+    bf16x8 qf[NT][KSQ];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int r = min(w.tile * TR + nt * 16 + r16, R - 1), t = r / a.G, g = r - t * a.G;
+        pos[nt] = base_pos + t;
+        const bf16* qp = a.q + (long)(w.q0 + t) * a.ldq + (long)(hk * a.G + g) * a.hd;
+        const bf16x8 z8 = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (int ks = 0; ks < KSQ; ++ks) {
+            // E4M3: a lane's 16 bytes of a K row are 16 channels, the operands of two products; the queries follow that order
+            const int ch = E4M3 ? (ks >> 1) * 64 + q4 * 16 + (ks & 1) * 8 : ks * 32 + q4 * 8;
+            const bf16x8 v = *(const bf16x8*)(qp + min(ch, a.hd - 8));
+            qf[nt][ks] = ch < a.hd ? v : z8;
+        }
+    }
+    const int pos_min = base_pos + w.tile * TR / a.G, pos_max = base_pos + min((w.tile * TR + TR - 1) / a.G, w.T - 1);
+    const bool one_pos = pos_min == pos_max;
+    const float c2 = a.scale * (E4M3 && a.k_scale ? a.k_scale[hk] : 1.f) * 1.4426950408889634f;
+
+    f32x4 o[NT][DT];
+    float m_run[NT], l_run[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        m_run[nt] = -INFINITY; l_run[nt] = 0.f;
+#pragma unroll
+        for (int i = 0; i < DT; ++i) o[nt][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+
+    constexpr int ES = E4M3 ? 1 : 2;
+    const long head_bytes = ((long)a.hd << a.lps) * ES;     // one head of one page
+    const char* kp = (const char*)a.k_pages + hk * head_bytes;
+    const char* vp = (const char*)a.v_pages + hk * head_bytes;
+    const long page_bytes = head_bytes * a.kv_heads;
+    const int* table = a.table + (long)w.seq * a.max_blocks;
+    const int P1 = (1 << a.lps) - 1;
+    u32x4 kreg[2][NK], vreg[NV];
+    bool page_ok[2];
+    // a block's two tiles of sixteen keys: their pages (an entry that is no page is read as page 0 and masked)
+    auto tile_off = [&](int key0, bool* ok) -> long {
+        const int blk = min(key0 >> a.lps, a.max_blocks - 1);
+        const int page = __builtin_amdgcn_readfirstlane(table[blk]);
+        *ok = (unsigned)page < (unsigned)a.n_pages;
+        return (*ok ? page : 0) * page_bytes + (long)(key0 & P1) * a.hd * ES;
+    };
+    long off[2];
+    auto load_v = [&]() {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int idx = i * 64 + lane, row = idx / VCH, ch = idx % VCH;
+            const long ro = (row < 16 ? off[0] : off[1]) + (long)(row & 15) * a.hd * ES;
+            vreg[i] = *(const u32x4*)(vp + ro + min(ch * 16, a.hd * ES - 16));
+        }
+    };
+    auto load_k = [&]() {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int i = 0; i < NK; ++i) {
+                const int cb = (i * 4 + q4) * 16;           // byte of the row
+                kreg[kt][i] = *(const u32x4*)(kp + off[kt] + (long)r16 * a.hd * ES + min(cb, a.hd * ES - 16));
+            }
+    };
+    bf16* vs = Vs[wave];
+    const int k_end = min(sp.hi, sp.first + b1 * 64);
+    int key0 = sp.first + b0 * 64 + wave * 32;
+    if (key0 < k_end) {
+        off[0] = tile_off(key0, &page_ok[0]); off[1] = tile_off(key0 + 16, &page_ok[1]);
+        load_v(); load_k();
+    }
+    for (; key0 < k_end; key0 += 128) {
+        const bool ok0 = page_ok[0], ok1 = page_ok[1];
+        const bool plain = ok0 && ok1 && key0 + 31 <= pos_min && key0 + 31 < k_end && (!a.window || key0 > pos_max - a.window);
+        // ---- V to LDS; rows that no row of the tile sees become zero (their bytes may be anything)
+        bool odd = false;                                   // a value that is not finite in a row that some see and others do not
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int idx = i * 64 + lane, row = idx / VCH, ch = idx % VCH;
+            bf16x8 v0, v1;
+            if constexpr (E4M3) { v0 = e4m3x8(vreg[i][0], vreg[i][1]); v1 = e4m3x8(vreg[i][2], vreg[i][3]); }
+            else v0 = __builtin_bit_cast(bf16x8, vreg[i]);
+            const bool pad = ch * 16 >= a.hd * ES;
+            bool none = pad;
+            if (!plain) {
+                const int j = key0 + row;
+                none |= j >= k_end || j < sp.lo || !(row < 16 ? ok0 : ok1);
+                if (!none && !one_pos) { odd |= nonfinite(v0); if constexpr (E4M3) odd |= nonfinite(v1); }
+            }
+            const bf16x8 z8 = {0, 0, 0, 0, 0, 0, 0, 0};
+            if constexpr (E4M3) {
+                *(bf16x8*)&vs[row * VST + ch * 16] = none ? z8 : v0;
+                *(bf16x8*)&vs[row * VST + ch * 16 + 8] = none ? z8 : v1;
+            } else *(bf16x8*)&vs[row * VST + ch * 8] = none ? z8 : v0;
+        }
+        asm volatile("" ::: "memory");
+        const int kn = key0 + 128;
+        if (kn < k_end) {
+            off[0] = tile_off(kn, &page_ok[0]); off[1] = tile_off(kn + 16, &page_ok[1]);
+            load_v();
+        }
+        // ---- scores: s[nt][kt][e] is row r16's with key key0 + 16 kt + 4 q4 + e
+        f32x4 s[NT][2];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) s[nt][kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < NK; ++i) {
+                bf16x8 k0, k1;
+                if constexpr (E4M3) { k0 = e4m3x8(kreg[kt][i][0], kreg[kt][i][1]); k1 = e4m3x8(kreg[kt][i][2], kreg[kt][i][3]); }
+                else k0 = __builtin_bit_cast(bf16x8, kreg[kt][i]);
+                if (a.hd < D) {                             // channels past the head: whatever was read there
+                    const bf16x8 z8 = {0, 0, 0, 0, 0, 0, 0, 0};
+                    if ((i * 4 + q4) * 16 >= a.hd * ES) { k0 = z8; if constexpr (E4M3) k1 = z8; }
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    if constexpr (E4M3) {
+                        s[nt][kt] = mfma16(k0, qf[nt][2 * i], s[nt][kt]);
+                        s[nt][kt] = mfma16(k1, qf[nt][2 * i + 1], s[nt][kt]);
+                    } else s[nt][kt] = mfma16(k0, qf[nt][i], s[nt][kt]);
+                }
+            }
+        }
+        if (kn < k_end) load_k();
+        const bool any_odd = !plain && !one_pos && __any(odd);
+        bf16x8 ph[NT], pl[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            if (!plain) {
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int j = key0 + kt * 16 + 4 * q4 + e;
+                        const bool see = j <= pos[nt] && j < k_end && (kt ? ok1 : ok0) && (!a.window || j > pos[nt] - a.window);
+                        s[nt][kt][e] = see ? s[nt][kt][e] : -INFINITY;
+                    }
+            }
+            float mx = fmaxf(fmaxf(fmaxf(s[nt][0][0], s[nt][0][1]), fmaxf(s[nt][0][2], s[nt][0][3])),
+                             fmaxf(fmaxf(s[nt][1][0], s[nt][1][1]), fmaxf(s[nt][1][2], s[nt][1][3])));
+            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const float m_new = fmaxf(m_run[nt], mx * c2);
+            const float ref = m_new == -INFINITY ? 0.f : m_new;           // a row that has seen nothing yet: 2^(-inf) = 0 throughout
+            const float alpha = __builtin_amdgcn_exp2f(m_run[nt] - ref);
+            float psum = 0.f;
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nt][kt][e], c2, -ref));
+                    psum += p;
+                    const bf16 hi = f2bf(p);
+                    ph[nt][kt * 4 + e] = hi;
+                    pl[nt][kt * 4 + e] = f2bf(p - bf2f(hi));
+                }
+            m_run[nt] = m_new;
+            l_run[nt] = l_run[nt] * alpha + psum;
+#pragma unroll
+            for (int i = 0; i < DT; ++i) o[nt][i] *= alpha;
+        }
+        // ---- O^T += V^T P^T: slot (q4, e) is key 4 q4 + e of the first tile, of the second from e = 4
+        const int vrow = 4 * q4 + (r16 >> 2), vcol = 4 * (r16 & 3);
+        if (!any_odd) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(&vs[vrow * VST + dt * 16 + vcol]));
+                const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(&vs[(16 + vrow) * VST + dt * 16 + vcol]));
+                const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    o[nt][dt] = mfma16(vf, ph[nt], o[nt][dt]);
+                    o[nt][dt] = mfma16(vf, pl[nt], o[nt][dt]);
+                }
+            }
+        } else {
+            // 0 * inf would carry a value into rows that do not see its key: each position's rows on their own, with the keys they see
+            for (int p = pos_min; p <= pos_max; ++p) {
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(&vs[vrow * VST + dt * 16 + vcol]));
+                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(&vs[(16 + vrow) * VST + dt * 16 + vcol]));
+                    bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int j = key0 + (e >> 2) * 16 + 4 * q4 + (e & 3);
+                        if (j > p || (a.window && j <= p - a.window)) vf[e] = 0;
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        f32x4 t = mfma16(vf, ph[nt], o[nt][dt]);
+                        t = mfma16(vf, pl[nt], t);
+                        o[nt][dt] = pos[nt] == p ? t : o[nt][dt];
+                    }
+                }
+            }
+        }
+        asm volatile("" ::: "memory");
+    }
+
+    // ---- merge the four waves: O of the sixteen rows of a tile in LDS, one after the other
+    constexpr int OST = D + 4;
+    static_assert(4 * 16 * OST * 4 <= (int)sizeof(Vs), "the merge uses V's LDS");
+    float* ob = (float*)&Vs[0][0];
+    const float vsc = E4M3 && a.v_scale ? a.v_scale[hk] : 1.f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        float l = l_run[nt];
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        __syncthreads();
+        if (q4 == 0) { sm[wave][r16] = m_run[nt]; sl[wave][r16] = l; }
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) *(f32x4*)&ob[(wave * 16 + r16) * OST + dt * 16 + 4 * q4] = o[nt][dt];
+        __syncthreads();
+        const int row = tid >> 4, c = (tid & 15) * (D / 16), r = w.tile * TR + nt * 16 + row;
+        float M = fmaxf(fmaxf(sm[0][row], sm[1][row]), fmaxf(sm[2][row], sm[3][row]));
+        const float ref = M == -INFINITY ? 0.f : M;
+        float acc[D / 16], lsum = 0.f;
+#pragma unroll
+        for (int e = 0; e < D / 16; ++e) acc[e] = 0.f;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const float f = __builtin_amdgcn_exp2f(sm[x][row] - ref);
+            lsum += sl[x][row] * f;
+#pragma unroll
+            for (int e = 0; e < D / 16; ++e) acc[e] += ob[(x * 16 + row) * OST + c + e] * f;
+        }
+        if (r < R) {
+            if (w.chunks == 1) {
+                const float inv = lsum > 0.f ? vsc / lsum : lsum == 0.f ? 0.f : lsum;          // a row that sees no key is zero; NaN stays
+                const int t = r / a.G, g = r - t * a.G;
+                bf16* op = a.out + (long)(w.q0 + t) * a.ldo + (long)(hk * a.G + g) * a.hd;
+#pragma unroll
+                for (int e = 0; e < D / 16; ++e) if (c + e < a.hd) op[c + e] = f2bf(acc[e] * inv);
+            } else {
+                const long pr = ((long)item * a.kv_heads + hk) * TR + nt * 16 + row;
+#pragma unroll
+                for (int e = 0; e < D / 16; ++e) a.part_o[pr * D + c + e] = acc[e];
+                if ((tid & 15) == 0) { a.part_ml[pr * 2] = M; a.part_ml[pr * 2 + 1] = lsum; }
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Joins the chunks of the rows of one token and key-value head.
+// ---------------------------------------------------------------------------------------------
+template <int D, int TR>
+__global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a, int e4m3) {
+    const int tok = blockIdx.x, hk = blockIdx.y;
+    __shared__ int first_s;
+    Work w;
+    if (!schedule<256, TR>(a, [&](int first, int items, Work* f) {
+            if (items == 0 || tok < f->q0 || tok >= f->q0 + f->T) return false;
+            first_s = first;
+            return true;
+        }, &w)) return;
+    if (w.chunks == 1) return;
+    const int t = max(tok - w.q0, 0), LPR = D / 4, lane = threadIdx.x % LPR;
+    const float vsc = e4m3 && a.v_scale ? a.v_scale[hk] : 1.f;
+    for (int g = threadIdx.x / LPR; g < a.G; g += 256 / LPR) {
+        const int r = t * a.G + g, tile = r / TR;
+        const Span sp = tile_span(a, w, tile, TR);
+        const int item = min(first_s + tile * w.chunks, a.grid_items - 1);           // (a cu that is no running sum: still in bounds)
+        const int chunks = min(max(1, (sp.nb + sp.S - 1) / sp.S), a.grid_items - item);
+        const long step = (long)a.kv_heads * TR, p0 = ((long)item * a.kv_heads + hk) * TR + (r - tile * TR);
+        float M = -INFINITY;
+        for (int c = 0; c < chunks; ++c) M = fmaxf(M, a.part_ml[(p0 + c * step) * 2]);
+        const float ref = M == -INFINITY ? 0.f : M;
+        float l = 0.f;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int c = 0; c < chunks; ++c) {
+            const float f = __builtin_amdgcn_exp2f(a.part_ml[(p0 + c * step) * 2] - ref);
+            l += a.part_ml[(p0 + c * step) * 2 + 1] * f;
+            const f32x4 v = *(const f32x4*)&a.part_o[(p0 + c * step) * D + lane * 4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] += v[e] * f;
+        }
+        const float inv = l > 0.f ? vsc / l : l == 0.f ? 0.f : l;
+        bf16x4 ov = {f2bf(acc[0] * inv), f2bf(acc[1] * inv), f2bf(acc[2] * inv), f2bf(acc[3] * inv)};
+        if (lane * 4 < a.hd) *(bf16x4*)(a.out + (long)tok * a.ldo + (long)(hk * a.G + g) * a.hd + lane * 4) = ov;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+static int rows_of_tile(const PagedAttnArgs* a, int max_q) { return 16; }
+static int template_dim(const PagedAttnArgs* a) { return a->hd <= 64 ? 64 : 128; }
+
+size_t paged_partial_floats(const PagedAttnArgs* a) { return (size_t)a->grid_items * a->kv_heads * a->tile_rows * template_dim(a); }
+
+size_t paged_attention_plan(PagedAttnArgs* a, int n_cus, int max_q, int max_len) {
+    const int TR = a->tile_rows = rows_of_tile(a, max_q);
+    const long tiles = (long)a->n_tokens * a->G / TR + a->n;              // of one key-value head, at most
+    a->target = (4 * n_cus + a->kv_heads - 1) / a->kv_heads;              // four workgroups a CU
+    a->min_blocks = 2;                                                    // 128 keys: one block of 32 for each of the four waves
+    long cap = (long)a->max_blocks << a->lps;
+    if (max_len > 0 && max_len < cap) cap = max_len;
+    const long nb = (cap + 63) / 64;
+    a->cmax = (int)(nb / a->min_blocks < 1 ? 1 : nb / a->min_blocks);
+    const long by_split = a->target + a->target / 1024 + 8 + tiles, by_len = tiles * a->cmax;
+    a->grid_items = (int)(by_len < by_split ? by_len : by_split);
+    if (a->cmax == 1) return 0;
+    return (paged_partial_floats(a) + (size_t)a->grid_items * a->kv_heads * TR * 2) * sizeof(float);
+}
+
+template <int D>
+static hipError_t launch(const PagedAttnArgs* a, int e4m3, int max_q, hipStream_t st) {
+    const dim3 grid(a->grid_items, a->kv_heads);
+    if (e4m3) paged_attn_rows_kernel<D, true, 1><<<grid, 256, 0, st>>>(*a);
+    else paged_attn_rows_kernel<D, false, 1><<<grid, 256, 0, st>>>(*a);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && a->cmax > 1) {
+        paged_attn_join_kernel<D, 16><<<dim3(a->n_tokens, a->kv_heads), 256, 0, st>>>(*a, e4m3);
+        e = hipGetLastError();
+    }
+    return e;
+}
+hipError_t paged_attention(const PagedAttnArgs* a, int e4m3, int max_q, hipStream_t st) {
+    return template_dim(a) == 64 ? launch<64>(a, e4m3, max_q, st) : launch<128>(a, e4m3, max_q, st);
+}

@@ -1,0 +1,206 @@
+// Block tables and slot maps of the paged key-value cache, on the device: which pages a sequence owns, and where each new token goes.
+//
+// reserve:  request i has c_i new tokens behind the len_i its sequence holds.  It needs ceil((len_i + c_i) / P) - ceil(len_i / P) pages; the
+//           requests' needs, summed in order, say which entries of the free list they take, counted from its end.  Token t of request i
+//           has position len_i + t and slot page(position / P) * P + position % P.
+// truncate: the pages behind the first ceil(new_len / P) go back to the free list, in the order in which a reserve of the same requests
+//           takes them: a truncate to the old lengths leaves the list as it was before the reserve, entry by entry.
+//
+// One workgroup does a call: the work is a prefix sum over the requests and a few words per page and token, and what bounds it is the chain
+// sequence -> length -> sum -> free entry -> store, each link a trip to the L2 or memory.  All requests are looked at before anything is
+// written, so a call that cannot be done (status) changes nothing.  Pages and tokens are dealt out flat, a thread finds the request of its
+// page or token by bisection of the sums in LDS: a request of two thousand tokens does not keep one thread busy.
+#include "paged.h"
+
+struct Scan2 { int a, b; };
+
+// inclusive prefix sums of two numbers over the workgroup; totals in *all
+static __device__ __forceinline__ Scan2 block_scan(Scan2 x, Scan2* wsum, Scan2* all) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int a = __shfl_up(x.a, o, 64), b = __shfl_up(x.b, o, 64);
+        if (lane >= o) { x.a += a; x.b += b; }
+    }
+    __syncthreads();                                          // wsum of an earlier scan has been read
+    if (lane == 63) wsum[wave] = x;
+    __syncthreads();
+    Scan2 before = {0, 0}, sum = {0, 0};
+    for (int w = 0; w < waves; ++w) {
+        if (w == wave) before = sum;
+        sum.a += wsum[w].a; sum.b += wsum[w].b;
+    }
+    *all = sum;
+    x.a += before.a; x.b += before.b;
+    return x;
+}
+
+// first i in [0, n) with end[i] > x (end is a running sum, its last value > x)
+static __device__ __forceinline__ int bisect(const int* end, int n, int x) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (end[mid] > x) hi = mid; else lo = mid + 1;
+    }
+    return lo;
+}
+
+#define PT_THREADS 1024
+struct Request { int seq, len, count, had, need, err; };     // had: pages it keeps; need: pages it takes (gives back)
+
+// What request i asks for; an entry with a negative sequence is padding and asks for nothing.
+template <bool RESERVE>
+static __device__ __forceinline__ Request look(const PagedReserveArgs& a, int i) {
+    Request r = {-1, 0, 0, 0, 0, 0};
+    if (i >= a.n) return r;
+    r.seq = a.seqs[i];
+    const int c = a.counts[i];
+    if (r.seq < 0) return r;
+    if (r.seq >= a.t.max_seqs) { r.seq = -1; r.err = PAGED_BAD_SEQ; return r; }
+    r.len = a.t.lens[r.seq];
+    const int lps = a.t.lps;
+    const long cap = (long)a.t.max_blocks << lps;
+    if (r.len < 0 || r.len > cap) { r.err = PAGED_BAD_SEQ; return r; }
+    const int P1 = (1 << lps) - 1;
+    if (RESERVE) {
+        if (c < 0) { r.err = PAGED_BAD_COUNT; return r; }
+        if ((long)r.len + c > cap) { r.err = PAGED_TOO_LONG; return r; }
+        r.count = c;
+        r.had = (int)(((long)r.len + P1) >> lps);
+        r.need = (int)(((long)r.len + c + P1) >> lps) - r.had;
+    } else {
+        if (c < 0 || c > r.len) { r.err = PAGED_BAD_COUNT; return r; }
+        r.count = c;
+        r.had = (int)(((long)c + P1) >> lps);
+        r.need = (int)(((long)r.len + P1) >> lps) - r.had;
+    }
+    return r;
+}
+
+template <bool RESERVE>
+__global__ __launch_bounds__(PT_THREADS) void paged_tables_kernel(PagedReserveArgs a, int map_tokens) {
+    __shared__ unsigned seen[PAGED_MAX_SEQS / 32];
+    __shared__ Scan2 wsum[PT_THREADS / 64];
+    __shared__ int pend[PT_THREADS], tend[PT_THREADS], rseq[PT_THREADS], rhad[PT_THREADS], rlen[PT_THREADS];
+    __shared__ int err_s;
+    __shared__ unsigned long long pages_s, tokens_s;
+    const int tid = threadIdx.x, NT = blockDim.x;
+    const PagedTables& t = a.t;
+    const int words = (t.max_seqs + 31) >> 5;
+    for (int i = tid; i < words; i += NT) seen[i] = 0;
+    if (tid == 0) { err_s = 0; pages_s = 0; tokens_s = 0; }
+    const int n_free = min(max(*t.n_free, 0), t.n_pages);
+    Request r0 = look<RESERVE>(a, tid);                        // kept: with at most NT requests nothing is read twice
+    __syncthreads();
+
+    // ---- look at every request
+    int err = 0;
+    unsigned long long pages = 0, tokens = 0;
+    for (int i0 = 0; i0 < a.n; i0 += NT) {
+        const Request r = i0 ? look<RESERVE>(a, i0 + tid) : r0;
+        err |= r.err;
+        if (r.seq >= 0) {
+            const unsigned bit = 1u << (r.seq & 31);
+            if (atomicOr(&seen[r.seq >> 5], bit) & bit) err |= PAGED_TWICE;
+        }
+        pages += r.need; tokens += RESERVE ? r.count : 0;
+    }
+    if (err) atomicOr(&err_s, err);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) { pages += __shfl_xor(pages, o, 64); tokens += __shfl_xor(tokens, o, 64); }
+    if ((tid & 63) == 0) { atomicAdd(&pages_s, pages); atomicAdd(&tokens_s, tokens); }
+    __syncthreads();
+    err = err_s; pages = pages_s; tokens = tokens_s;
+    unsigned long long missing = 0;
+    if (err) {                                                 // the sums of requests that are none say nothing
+    } else if (RESERVE) {
+        if (pages > (unsigned long long)n_free) { err |= PAGED_NO_PAGES; missing = pages - n_free; }
+        if (tokens > (unsigned long long)a.n_tokens) err |= PAGED_MANY_TOKENS;
+    } else if (pages + n_free > (unsigned long long)t.n_pages) err |= PAGED_BAD_SEQ;       // more pages than the pool has: the tables are not its own
+    if (tid == 0) {
+        a.status[0] = err;
+        a.status[1] = missing > 0x7fffffffull ? 0x7fffffff : (int)missing;
+    }
+    if (err) {                                                 // uniform: nothing is taken, every token goes nowhere
+        if (RESERVE) {
+            for (int i = tid; i <= a.n; i += NT) a.cu[i] = 0;
+            for (int i = tid; i < a.n_tokens; i += NT) { a.slots[i] = -1; a.positions[i] = -1; }
+        }
+        return;
+    }
+
+    // ---- deal out pages and tokens
+    Scan2 base = {0, 0};
+    for (int i0 = 0; i0 < a.n; i0 += NT) {
+        const Request r = i0 ? look<RESERVE>(a, i0 + tid) : r0;
+        Scan2 all;
+        const Scan2 in = block_scan({r.need, RESERVE ? r.count : 0}, wsum, &all);
+        pend[tid] = in.a; tend[tid] = in.b; rseq[tid] = r.seq; rhad[tid] = r.had; rlen[tid] = r.len;
+        if (RESERVE && i0 + tid < a.n) {
+            a.cu[i0 + tid + 1] = base.b + in.b;
+            if (i0 + tid == 0) a.cu[0] = 0;
+        }
+        __syncthreads();
+        const int m = min(NT, a.n - i0);
+        for (int p = tid; p < all.a; p += NT) {
+            const int i = bisect(pend, m, p);
+            const int k = p - (i ? pend[i - 1] : 0);
+            int* e = t.table + (long)rseq[i] * t.max_blocks + rhad[i] + k;
+            if (RESERVE) *e = t.free_pages[n_free - 1 - (base.a + p)];
+            else { t.free_pages[n_free + (int)pages - 1 - (base.a + p)] = *e; *e = -1; }
+        }
+        if (RESERVE && map_tokens)
+            for (int x = tid; x < all.b; x += NT) {
+                const int i = bisect(tend, m, x), off = x - (i ? tend[i - 1] : 0);
+                const int pos = rlen[i] + off, blk = pos >> t.lps;
+                const int page = blk < rhad[i] ? t.table[(long)rseq[i] * t.max_blocks + blk]
+                                               : t.free_pages[n_free - 1 - (base.a + (i ? pend[i - 1] : 0) + blk - rhad[i])];
+                a.positions[base.b + x] = pos;
+                a.slots[base.b + x] = (unsigned)page < (unsigned)t.n_pages ? (page << t.lps) + (pos & ((1 << t.lps) - 1)) : -1;
+            }
+        if (r.seq >= 0) t.lens[r.seq] = RESERVE ? r.len + r.count : r.count;
+        base.a += all.a; base.b += all.b;
+        __syncthreads();
+    }
+    if (RESERVE && map_tokens)
+        for (int x = base.b + tid; x < a.n_tokens; x += NT) { a.slots[x] = -1; a.positions[x] = -1; }
+    if (RESERVE && a.n == 0 && tid == 0) a.cu[0] = 0;
+    if (tid == 0) *t.n_free = RESERVE ? n_free - base.a : n_free + base.a;
+}
+
+// The slots of many tokens, behind the tables kernel and over the whole chip: token x belongs to the request whose cu range holds it, and its
+// sequence ends (now) at lens[seq].
+__global__ __launch_bounds__(256) void paged_slots_kernel(PagedReserveArgs a) {
+    const int x = blockIdx.x * 256 + threadIdx.x;
+    if (x >= a.n_tokens) return;
+    const PagedTables& t = a.t;
+    if (a.status[0]) return;                                   // the tables kernel has written them
+    int slot = -1, pos = -1;
+    if (x < a.cu[a.n]) {
+        const int i = bisect(a.cu + 1, a.n, x);
+        const int seq = a.seqs[i];
+        pos = t.lens[seq] - (a.cu[i + 1] - x);
+        const int page = t.table[(long)seq * t.max_blocks + (pos >> t.lps)];
+        if ((unsigned)page < (unsigned)t.n_pages) slot = (page << t.lps) + (pos & ((1 << t.lps) - 1));
+    }
+    a.slots[x] = slot;
+    a.positions[x] = pos;
+}
+
+static int threads_for(int work) { return work <= 256 ? 256 : work <= 512 ? 512 : PT_THREADS; }
+
+hipError_t paged_reserve(const PagedReserveArgs* a, hipStream_t st) {
+    const int map = a->n_tokens <= 4 * PT_THREADS;             // four tokens a thread: beyond that a second launch over the chip
+    const int work = a->n > a->n_tokens || !map ? a->n : a->n_tokens;
+    paged_tables_kernel<true><<<1, threads_for(work), 0, st>>>(*a, map);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && !map) {
+        paged_slots_kernel<<<(a->n_tokens + 255) / 256, 256, 0, st>>>(*a);
+        e = hipGetLastError();
+    }
+    return e;
+}
+hipError_t paged_truncate(const PagedReserveArgs* a, hipStream_t st) {
+    paged_tables_kernel<false><<<1, threads_for(a->n), 0, st>>>(*a, 0);
+    return hipGetLastError();
+}

@@ -30,11 +30,17 @@ class TensorView(C.Structure):
                 ("reserved", C.c_int32)]
 
 
+class PagedDesc(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k_pages", "v_pages", "block_table", "lens", "free_pages", "n_free", "k_scale", "v_scale")] + \
+               [(n, C.c_int32) for n in ("layers", "n_pages", "page_size", "kv_heads", "head_dim", "kv_type", "max_seqs", "max_blocks")]
+
+
+KV_BF16, KV_E4M3 = 0, 1
 CACHE_NONE, CACHE_SINK, CACHE_SLIDING, CACHE_STATIC = 0, 1, 2, 3
 ATTN_TRAILING, ATTN_HF449_SDPA, ATTN_FA2 = 0, 1, 2
 
 # every symbol include/aha_amd.h declares: (name, restype, argtypes)
-_P, _I, _F = C.c_void_p, C.c_int, C.c_float
+_P, _I, _F, _L = C.c_void_p, C.c_int, C.c_float, C.c_int64
 SYMBOLS = [
     ("aha_ctx_create", _I, [C.POINTER(ModelDesc), _I, C.POINTER(_P)]),
     ("aha_ctx_load_weights", _I, [_P, C.POINTER(TensorView), C.c_size_t, _P]),
@@ -93,6 +99,14 @@ SYMBOLS = [
     ("aha_allgather_scores", _I, [_P, _P, _I, _P, _P]),
     ("aha_comm_destroy", None, [_P]),
     ("aha_comm_last_error", C.c_char_p, []),
+    ("aha_paged_create", _I, [C.POINTER(PagedDesc), _I, C.POINTER(_P)]),
+    ("aha_paged_destroy", None, [_P]),
+    ("aha_paged_last_error", C.c_char_p, []),
+    ("aha_paged_reserve", _I, [_P, _P, _P, _I, _P, _P, _I, _P, _P, _P]),
+    ("aha_paged_truncate", _I, [_P, _P, _P, _I, _P, _P]),
+    ("aha_paged_append", _I, [_P, _I, _P, _L, _I, _P, _L, _P, _L, _P, _L, _P, _P, _I, _P, _P, _I, _P]),
+    ("aha_paged_attention_workspace", _I, [_P, _I, _I, _I, _I, _I, C.POINTER(C.c_size_t)]),
+    ("aha_paged_attention", _I, [_P, _I, _P, _L, _I, _P, _P, _I, _I, _I, _I, _I, _F, _P, _L, _P, C.c_size_t, _P]),
 ]
 EPI_SPLITK_F32, EPI_BF16, EPI_SWIGLU, EPI_F32 = 0, 1, 2, 3
 ACT_NONE, ACT_GELU_TANH, ACT_GELU_ERF, ACT_QUICK_GELU = 0, 1, 2, 3

@@ -179,6 +179,15 @@ class Runtime:
                     capacity: Optional[int] = None, attn_semantics: str = "trailing") -> Stream:
         return Stream(self, alt_cache, window_length, num_sink_tokens, capacity or self.desc.max_positions, attn_semantics)
 
+    def open_paged(self, n_pages: int, max_seqs: int, *, page_size: int = 64, max_blocks: Optional[int] = None,
+                   dtype: torch.dtype = torch.bfloat16, **tensors):
+        """A paged key-value cache (aha_amd.paged.PagedKVCache) for this model: its layers, key-value heads and RoPE table; max_blocks pages a
+        sequence (default: the table's positions).  `tensors`: scales or storage of the caller's."""
+        from .paged import PagedKVCache
+        d = self.desc
+        return PagedKVCache(n_pages, page_size, d.kv_heads, d.head_dim, max_seqs, max_blocks or -(-d.max_positions // page_size), layers=d.layers, dtype=dtype,
+                            device=self.device, rope=tuple(t.to(self.device) for t in self._rope_cpu), **tensors)
+
     def set_rerotation_table(self, s: Stream, T: int):
         """Optional: install a host-computed SinkCache re-rotation table for (window, n_sink, T).  aha_lm_step builds the same
         table on the device, asynchronously, the first time a combination evicts, so the step path never calls this; it

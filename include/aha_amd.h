@@ -329,6 +329,63 @@ int aha_pool_forward(aha_ctx* ctx, const void* in, int n_frames, int grid, int o
 int aha_pool_gather_rows_forward(aha_ctx* ctx, const void* in, int n_frames, int grid, int out_grid, int channels, int frame_rows, void* out,
                                  aha_hip_stream st);
 
+/* ---- paged key-value cache: the K / V of many sequences in ONE pool of pages.  Next to the ring caches of aha_stream_* (a contiguous
+ * buffer per stream at its full capacity) it serves requests that come and go and grow to unknown lengths: a sequence owns only the pages
+ * it fills, any number of requests run in one call, and lengths and tables live on the device, so a step needs no host round trip and can
+ * be captured into a graph.  All device memory is the caller's; the handle holds the description only.  The calls enqueue on the given
+ * stream, on the pool's device whatever the current one is, and never synchronise or allocate.  A handle may be used from several threads;
+ * calls that change the tables of one pool must be ordered by the caller (one stream, or events).
+ * One step:  reserve (pages, slots, positions)  ->  per layer: append (rotate, store)  ->  attention.  aha_paged_last_error: the message of
+ * the calling thread's last refused call. ------------------------------------------------------------------------------------------------ */
+typedef struct aha_paged aha_paged;
+enum { AHA_KV_BF16 = 0, AHA_KV_E4M3 = 1 };   /* type of the pages.  E4M3 (OCP): page value = round(clamp(x / scale, +-448)), x ~ value * scale */
+typedef struct aha_paged_desc {
+    void *k_pages, *v_pages;                  /* [layers][n_pages][kv_heads][page_size][head_dim], aligned to 16 bytes */
+    int32_t* block_table;                     /* [max_seqs][max_blocks]: page of each run of page_size tokens; entries behind the last are ignored */
+    int32_t* lens;                            /* [max_seqs]: tokens of each sequence */
+    int32_t *free_pages, *n_free;             /* [n_pages], [1]: the free list is free_pages[0 .. *n_free) and is taken from its end */
+    const float *k_scale, *v_scale;           /* [layers][kv_heads], E4M3 only; null = 1 */
+    int32_t layers, n_pages, page_size;       /* page_size: a power of two, 16 .. 1024 */
+    int32_t kv_heads, head_dim;               /* head_dim: a multiple of 16, at most 128 */
+    int32_t kv_type, max_seqs, max_blocks;    /* max_seqs <= 65536 */
+} aha_paged_desc;
+int aha_paged_create(const aha_paged_desc* desc, int device, aha_paged** out);
+void aha_paged_destroy(aha_paged* p);
+const char* aha_paged_last_error(void);
+/* Sequence seqs[i] grows by counts[i] tokens, i < n (a negative sequence is padding and its count ignored).  Pages are taken from the end of
+ * the free list in the order of the requests.  Out: cu_tokens [n+1], the running sum of the counts; slots / positions [n_tokens], of the
+ * new tokens of request 0, 1, ...: slot = page * page_size + place in the page, position = index in the sequence; -1 behind the last.
+ * status [2], on the device: [0] = 0 or a sum of AHA_PAGED_*, then NOTHING was changed, every slot is -1 and every cu_tokens 0 (append and
+ * attention with them do nothing); [1] = pages missing. */
+enum { AHA_PAGED_NO_PAGES = 1,     /* the free list is too short                         */
+       AHA_PAGED_MANY_TOKENS = 2,  /* the counts add up to more than n_tokens            */
+       AHA_PAGED_BAD_SEQ = 4,      /* a sequence >= max_seqs, or a corrupt length        */
+       AHA_PAGED_TWICE = 8,        /* a sequence is listed twice                         */
+       AHA_PAGED_TOO_LONG = 16,    /* a sequence would outgrow max_blocks pages          */
+       AHA_PAGED_BAD_COUNT = 32 }; /* a negative count; truncate: a length out of 0..len */
+int aha_paged_reserve(aha_paged* p, const int32_t* seqs, const int32_t* counts, int n, int32_t* slots, int32_t* positions, int n_tokens,
+                      int32_t* cu_tokens, int32_t* status, aha_hip_stream st);
+/* Sequence seqs[i] is cut to new_lens[i] <= its length (0: it is released); its pages behind the last needed one return to the free list and
+ * their table entries become -1.  The exact inverse of a reserve of the same sequences in the same order. */
+int aha_paged_truncate(aha_paged* p, const int32_t* seqs, const int32_t* new_lens, int n, int32_t* status, aha_hip_stream st);
+/* One layer's new tokens: q [n_tokens][heads][head_dim] and k are rotated by the row positions[t] (clamped to 0 .. n_pos-1) of cos / sin (bf16
+ * [n_pos][head_dim], the table of aha_ctx_set_rope_table; null: no rotation), q to q_out (may be q), k and v to the pages of their slots; a
+ * token with a slot outside the pool is not stored.  Rows have strides ld* in elements (multiples of 8), heads = 0: no queries.  fp32
+ * arithmetic, one rounding.  Two tokens of a call must not share a slot. */
+int aha_paged_append(aha_paged* p, int layer, const void* q, int64_t ldq, int heads, void* q_out, int64_t ldqo, const void* k, int64_t ldk,
+                     const void* v, int64_t ldv, const int32_t* slots, const int32_t* positions, int n_tokens, const void* cos, const void* sin,
+                     int n_pos, aha_hip_stream st);
+/* out[t] = softmax(scale * q[t] K^T) V, bf16 [n_tokens][heads][head_dim]: rows cu_tokens[i] .. cu_tokens[i+1]-1 are the LAST tokens of sequence
+ * seqs[i] (its keys are already appended) and see the keys at and before their position, the nearest `window` of them (0: all).  heads / kv_heads
+ * query heads share a key-value head.  A row that sees no key is 0; rows of padding (negative sequence) and behind cu_tokens[n] are left as
+ * they were.  A table entry that is no page hides its keys.  max_q, max_len: the most new tokens and keys of a request (0: not known); they choose the kernel
+ * and the split of long sequences, results are right for any value.  workspace: aha_paged_attention_workspace bytes for the same sizes,
+ * aligned to 16, used by this call only until its work is done (calls that may run at once need one each). */
+int aha_paged_attention_workspace(aha_paged* p, int heads, int n_tokens, int n, int max_q, int max_len, size_t* bytes);
+int aha_paged_attention(aha_paged* p, int layer, const void* q, int64_t ldq, int heads, const int32_t* seqs, const int32_t* cu_tokens, int n,
+                        int n_tokens, int max_q, int max_len, int window, float scale, void* out, int64_t ldo, void* workspace,
+                        size_t workspace_bytes, aha_hip_stream st);
+
 #ifdef __cplusplus
 }
 #endif
