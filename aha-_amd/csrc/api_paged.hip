@@ -173,6 +173,6 @@ extern "C" int aha_paged_attention(aha_paged* p, int layer, const void* q, int64
     a.window = window; a.scale = scale;
     a.part_o = (float*)workspace;
     a.part_ml = need ? a.part_o + paged_partial_floats(&a) : nullptr;
-    RUN("paged attention", paged_attention(&a, d.kv_type == AHA_KV_E4M3, max_q, (hipStream_t)st));
+    RUN("paged attention", paged_attention(&a, d.kv_type == AHA_KV_E4M3, (hipStream_t)st));
     return 0;
 }

@@ -52,4 +52,4 @@ hipError_t paged_append(const PagedAppendArgs* a, hipStream_t st);
 // fills target / min_blocks / cmax / grid_items for max_len keys at most and returns the bytes of partial results the call needs (0: no split)
 size_t paged_attention_plan(PagedAttnArgs* a, int n_cus, int max_q, int max_len);
 size_t paged_partial_floats(const PagedAttnArgs* a);          // floats of part_o; part_ml lies behind them
-hipError_t paged_attention(const PagedAttnArgs* a, int e4m3, int max_q, hipStream_t st);
+hipError_t paged_attention(const PagedAttnArgs* a, int e4m3, hipStream_t st);

@@ -16,6 +16,7 @@
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+typedef const __attribute__((address_space(4))) int* table_t;         // read by scalar loads: nothing writes the tables while a call runs
 
 // ---------------------------------------------------------------------------------------------
 // The split.  Request i: R_i = G * T_i rows in rt_i tiles of TR, at most nb_i blocks of 64 keys a tile.  With W = sum rt_i * nb_i blocks of
@@ -190,14 +191,14 @@ __global__ __launch_bounds__(256) void paged_attn_rows_kernel(PagedAttnArgs a) {
     const char* kp = (const char*)a.k_pages + hk * head_bytes;
     const char* vp = (const char*)a.v_pages + hk * head_bytes;
     const long page_bytes = head_bytes * a.kv_heads;
-    const int* table = a.table + (long)w.seq * a.max_blocks;
+    const table_t table = (table_t)(uintptr_t)(a.table + (long)w.seq * a.max_blocks);
     const int P1 = (1 << a.lps) - 1;
     u32x4 kreg[2][NK], vreg[NV];
     bool page_ok[2];
     // a block's two tiles of sixteen keys: their pages (an entry that is no page is read as page 0 and masked)
     auto tile_off = [&](int key0, bool* ok) -> long {
         const int blk = min(key0 >> a.lps, a.max_blocks - 1);
-        const int page = __builtin_amdgcn_readfirstlane(table[blk]);
+        const int page = table[blk];
         *ok = (unsigned)page < (unsigned)a.n_pages;
         return (*ok ? page : 0) * page_bytes + (long)(key0 & P1) * a.hd * ES;
     };
@@ -403,6 +404,282 @@ __global__ __launch_bounds__(256) void paged_attn_rows_kernel(PagedAttnArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------
+// Many rows (frames, prompts): bound by the matrix cores and the exponentials.  A workgroup's four waves have 32 rows each and share blocks of
+// 64 keys, K and V double-buffered in LDS: the next block is under way while this one is computed, with one barrier a block.  bf16 pages go
+// straight to LDS (global_load_lds, 1 KiB of contiguous rows an instruction), e4m3 through registers, where they become bf16.  In LDS a row's
+// 16-byte chunks are permuted by its number: sixteen rows read at one column, or eight rows at two, touch every bank once.
+// P is rounded to bf16 (half a step, 2^-8 of p, as the output itself is); the sum of the row is taken from the rounded values, by the matrix cores
+// (a product with ones), so that numerator and denominator round alike.  The running maximum moves only when a score exceeds it by 2^8: until
+// then the exponentials stay below 2^8 and neither the sum nor the output is rescaled.
+// ---------------------------------------------------------------------------------------------
+template <int D> struct TileLds {
+    static constexpr int CPR = D / 8, RPP = 64 / CPR;       // 16-byte chunks of a row; rows of a 1-KiB piece
+    static __device__ __forceinline__ int k_slot(int row, int ch) { return row * D + ((ch ^ (D == 128 ? row & 15 : (row >> 1) & 7)) << 3); }
+    static __device__ __forceinline__ int v_slot(int row, int ch) { return row * D + ((ch ^ (D == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3))) << 3); }
+};
+typedef const __attribute__((address_space(1))) unsigned* gptr_t;
+typedef __attribute__((address_space(3))) unsigned* lptr_t;
+
+template <int D, bool E4M3>
+__global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a) {
+    constexpr int KSQ = D / 32, DT = D / 16, TR = 128, BLK = 64 * D;
+    using LD = TileLds<D>;
+    extern __shared__ __attribute__((aligned(16))) bf16 kv[];             // [buffer][K, V][64][D]
+    __shared__ int odd_s[2];
+
+    const int item = blockIdx.x, hk = blockIdx.y;
+    Work w;
+    if (!schedule<256, TR>(a, [&](int first, int items, Work* f) {
+            const int k = item - first;
+            if (k < 0 || k >= items) return false;
+            f->tile = items / f->chunks - 1 - k / f->chunks;              // the longest rows of a prompt first
+            f->chunk = k % f->chunks;
+            return true;
+        }, &w)) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int q4 = lane >> 4, r16 = lane & 15;
+    w.seq = __builtin_amdgcn_readfirstlane(w.seq); w.q0 = __builtin_amdgcn_readfirstlane(w.q0);
+    w.T = __builtin_amdgcn_readfirstlane(w.T); w.L = __builtin_amdgcn_readfirstlane(w.L);
+    w.tile = __builtin_amdgcn_readfirstlane(w.tile); w.chunk = __builtin_amdgcn_readfirstlane(w.chunk);
+    w.chunks = __builtin_amdgcn_readfirstlane(w.chunks);
+    const Span sp = tile_span(a, w, w.tile, TR);
+    const int b0 = w.chunk * sp.S, b1 = min(sp.nb, b0 + sp.S);
+    if (b0 >= b1 && w.chunk) return;
+    const int R = w.T * a.G, base_pos = w.L - w.T;
+    const int row0 = w.tile * TR + wave * 32;
+    const bool wave_on = row0 < R;
+
+    int pos[2];
+    bf16x8 qf[2][KSQ];
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+        const int r = min(row0 + nt * 16 + r16, R - 1), t = r / a.G, g = r - t * a.G;
+        pos[nt] = base_pos + t;
+        const bf16* qp = a.q + (long)(w.q0 + t) * a.ldq + (long)(hk * a.G + g) * a.hd;
+        const bf16x8 z8 = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (int ks = 0; ks < KSQ; ++ks) {
+            const int ch = ks * 32 + q4 * 8;
+            const bf16x8 v = *(const bf16x8*)(qp + min(ch, a.hd - 8));
+            qf[nt][ks] = ch < a.hd ? v : z8;
+        }
+    }
+    // the positions of the workgroup's rows, and of the wave's
+    const int pos_lo = base_pos + w.tile * TR / a.G, pos_hi = base_pos + min((w.tile * TR + TR - 1) / a.G, w.T - 1);
+    const int wpos_lo = base_pos + min(row0, R - 1) / a.G, wpos_hi = base_pos + min(row0 + 31, R - 1) / a.G;
+    const float c2 = a.scale * (E4M3 && a.k_scale ? a.k_scale[hk] : 1.f) * 1.4426950408889634f;
+
+    f32x4 o[2][DT], lacc[2];
+    float m_run[2];
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+        m_run[nt] = -INFINITY; lacc[nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < DT; ++i) o[nt][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+
+    constexpr int ES = E4M3 ? 1 : 2;
+    const int row_bytes = a.hd * ES;
+    const long head_bytes = ((long)a.hd << a.lps) * ES, page_bytes = head_bytes * a.kv_heads;
+    const char* kp = (const char*)a.k_pages + hk * head_bytes;
+    const char* vp = (const char*)a.v_pages + hk * head_bytes;
+    const table_t table = (table_t)(uintptr_t)(a.table + (long)w.seq * a.max_blocks);
+    const int P1 = (1 << a.lps) - 1;
+    // the pages of a block's four tiles of sixteen keys (scalar loads; an entry that is no page is read as page 0 and masked); looked up two
+    // blocks ahead
+    auto look_up = [&](int key0, int i) { return table[min((key0 + 16 * i) >> a.lps, a.max_blocks - 1)]; };
+    auto no_page = [&](int page) { return (unsigned)page >= (unsigned)a.n_pages; };
+    constexpr int NL = E4M3 ? D / 64 : D / 32;              // 16-byte loads a lane of sixteen rows
+    u32x4 kreg[NL], vreg[NL];
+    auto stage = [&](int key0, int page, int buf) {         // wave w has keys 16 w .. 16 w + 15 of a block; bf16: into LDS; e4m3: into registers
+        page = no_page(page) ? 0 : page;
+        const long off = page * page_bytes + (long)((key0 + wave * 16) & P1) * row_bytes;
+        if constexpr (!E4M3) {
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                const int row = i * LD::RPP + lane / LD::CPR, c = lane % LD::CPR, rb = wave * 16 + row;
+                const int ck = (LD::k_slot(rb, c) - rb * D) * 2, cv = (LD::v_slot(rb, c) - rb * D) * 2;        // the chunk that belongs in this place
+                __builtin_amdgcn_global_load_lds((gptr_t)(kp + off + row * row_bytes + min(ck, row_bytes - 16)), (lptr_t)(kv + buf * 2 * BLK + (wave * 16 + i * LD::RPP) * D), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((gptr_t)(vp + off + row * row_bytes + min(cv, row_bytes - 16)), (lptr_t)(kv + buf * 2 * BLK + BLK + (wave * 16 + i * LD::RPP) * D), 16, 0, 0);
+            }
+        } else {
+            constexpr int C = D / 16;
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                const int idx = i * 64 + lane, row = idx / C, cb = min(idx % C * 16, row_bytes - 16);
+                kreg[i] = *(const u32x4*)(kp + off + row * row_bytes + cb);
+                vreg[i] = *(const u32x4*)(vp + off + row * row_bytes + cb);
+            }
+        }
+    };
+    auto unstage = [&](int buf) {                           // e4m3: from registers into LDS, as bf16
+        if constexpr (E4M3) {
+            constexpr int C = D / 16;
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                const int idx = i * 64 + lane, row = wave * 16 + idx / C, c = idx % C * 2;
+                *(bf16x8*)(kv + buf * 2 * BLK + LD::k_slot(row, c)) = e4m3x8(kreg[i][0], kreg[i][1]);
+                *(bf16x8*)(kv + buf * 2 * BLK + LD::k_slot(row, c + 1)) = e4m3x8(kreg[i][2], kreg[i][3]);
+                *(bf16x8*)(kv + buf * 2 * BLK + BLK + LD::v_slot(row, c)) = e4m3x8(vreg[i][0], vreg[i][1]);
+                *(bf16x8*)(kv + buf * 2 * BLK + BLK + LD::v_slot(row, c + 1)) = e4m3x8(vreg[i][2], vreg[i][3]);
+            }
+        }
+    };
+    const bf16 one = (bf16)1.0f;
+    const bf16x8 ones = {one, one, one, one, one, one, one, one};
+
+    int buf = 0;
+    // the wave's own page a block ahead; all four of the block itself, for the mask
+    int mine = look_up(sp.first + b0 * 64, wave);
+    int p0 = look_up(sp.first + b0 * 64, 0), p1 = look_up(sp.first + b0 * 64, 1), p2 = look_up(sp.first + b0 * 64, 2), p3 = look_up(sp.first + b0 * 64, 3);
+    if (b0 < b1) { stage(sp.first + b0 * 64, mine, 0); unstage(0); }
+    mine = look_up(sp.first + b0 * 64 + 64, wave);
+    for (int b = b0; b < b1; ++b, buf ^= 1) {
+        const int key0 = sp.first + b * 64;
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();                       // this block is in LDS, the other buffer is free
+        const unsigned bad = (no_page(p0) ? 1u : 0u) | (no_page(p1) ? 2u : 0u) | (no_page(p2) ? 4u : 0u) | (no_page(p3) ? 8u : 0u);
+        const bool plain = !bad && key0 + 63 <= pos_lo && (!a.window || key0 > pos_hi - a.window);             // every row sees every key
+        bool odd = false;
+        if (!plain) {
+            // values that no row of the workgroup sees become zero; is one that some see and others do not not finite?
+            if (tid == 0) odd_s[buf] = 0;
+            __syncthreads();
+            bool mine_odd = false;
+            for (int x = tid; x < 64 * LD::CPR; x += 256) {
+                const int row = x / LD::CPR, j = key0 + row;
+                bf16x8* vv = (bf16x8*)(kv + buf * 2 * BLK + BLK + x * 8);
+                if (j >= sp.hi || j < sp.lo || (bad >> (row >> 4) & 1)) *vv = (bf16x8){0, 0, 0, 0, 0, 0, 0, 0};
+                else mine_odd |= nonfinite(*vv);
+            }
+            if (mine_odd) odd_s[buf] = 1;
+            __syncthreads();
+            odd = odd_s[buf] != 0 && pos_lo != pos_hi;
+        }
+        if (b + 1 < b1) {
+            stage(key0 + 64, mine, buf ^ 1);
+            mine = look_up(key0 + 128, wave);
+            p0 = look_up(key0 + 64, 0); p1 = look_up(key0 + 64, 1); p2 = look_up(key0 + 64, 2); p3 = look_up(key0 + 64, 3);
+        }
+        // a wave whose rows see nothing of the block, or that has none, only keeps the barriers
+        if (wave_on && key0 <= wpos_hi && (!a.window || key0 + 63 > wpos_lo - a.window)) {
+            const bf16* ks_ = kv + buf * 2 * BLK;
+            const bf16* vs_ = ks_ + BLK;
+            f32x4 s[2][4];
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt) {
+                s[0][kt] = s[1][kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int ks = 0; ks < KSQ; ++ks) {
+                    const bf16x8 kf = *(const bf16x8*)&ks_[LD::k_slot(kt * 16 + r16, ks * 4 + q4)];
+                    s[0][kt] = mfma16(kf, qf[0][ks], s[0][kt]);
+                    s[1][kt] = mfma16(kf, qf[1][ks], s[1][kt]);
+                }
+            }
+            const bool masked = !plain && (bad || key0 + 63 > wpos_lo || (a.window && key0 <= wpos_hi - a.window));
+            bf16x8 pb[2][2];
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt) {
+                if (masked) {
+#pragma unroll
+                    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int j = key0 + kt * 16 + 4 * q4 + e;
+                            const bool see = j <= pos[nt] && !(bad >> kt & 1) && (!a.window || j > pos[nt] - a.window);
+                            s[nt][kt][e] = see ? s[nt][kt][e] : -INFINITY;
+                        }
+                }
+                float mx = fmaxf(fmaxf(s[nt][0][0], s[nt][0][1]), fmaxf(s[nt][0][2], s[nt][0][3]));
+#pragma unroll
+                for (int kt = 1; kt < 4; ++kt) mx = fmaxf(mx, fmaxf(fmaxf(s[nt][kt][0], s[nt][kt][1]), fmaxf(s[nt][kt][2], s[nt][kt][3])));
+                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                mx *= c2;
+                if (__any(mx > m_run[nt] + 8.f)) {          // (-inf + 8 = -inf: the first key a row sees sets its reference)
+                    const float m_new = mx > m_run[nt] + 8.f ? mx : m_run[nt];
+                    const float alpha = m_new == m_run[nt] ? 1.f : __builtin_amdgcn_exp2f(m_run[nt] - m_new);
+                    m_run[nt] = m_new;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) lacc[nt][e] *= alpha;
+#pragma unroll
+                    for (int i = 0; i < DT; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[nt][i][e] *= alpha;
+                }
+                const float ref = m_run[nt] == -INFINITY ? 0.f : -m_run[nt];
+#pragma unroll
+                for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        pb[nt][kt >> 1][(kt & 1) * 4 + e] = f2bf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[nt][kt][e], c2, ref)));
+#pragma unroll
+                for (int kp_ = 0; kp_ < 2; ++kp_) lacc[nt] = mfma16(ones, pb[nt][kp_], lacc[nt]);
+            }
+            // O^T += V^T P^T: slot (q4, e) of a pair of key tiles is key 4 q4 + e of the first, of the second from e = 4
+            const int vrow = 4 * q4 + (r16 >> 2), vch = (r16 & 3) >> 1, vin = 4 * (r16 & 1);
+            auto v_frag = [&](int dt, int kp_) {
+                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(vs_ + LD::v_slot(kp_ * 32 + vrow, dt * 2 + vch) + vin));
+                const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(vs_ + LD::v_slot(kp_ * 32 + 16 + vrow, dt * 2 + vch) + vin));
+                return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            };
+            if (!odd) {
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int kp_ = 0; kp_ < 2; ++kp_) {
+                        const bf16x8 vf = v_frag(dt, kp_);
+                        o[0][dt] = mfma16(vf, pb[0][kp_], o[0][dt]);
+                        o[1][dt] = mfma16(vf, pb[1][kp_], o[1][dt]);
+                    }
+            } else {
+                for (int p = wpos_lo; p <= wpos_hi; ++p) {  // each position's rows on their own, with the keys they see (0 * inf is no zero)
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                        for (int kp_ = 0; kp_ < 2; ++kp_) {
+                            bf16x8 vf = v_frag(dt, kp_);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const int j = key0 + kp_ * 32 + (e >> 2) * 16 + 4 * q4 + (e & 3);
+                                if (j > p || (a.window && j <= p - a.window)) vf[e] = 0;
+                            }
+#pragma unroll
+                            for (int nt = 0; nt < 2; ++nt) {
+                                const f32x4 x = mfma16(vf, pb[nt][kp_], o[nt][dt]);
+                                o[nt][dt] = pos[nt] == p ? x : o[nt][dt];
+                            }
+                        }
+                }
+            }
+        }
+        if (b + 1 < b1) unstage(buf ^ 1);
+    }
+    if (!wave_on) return;
+
+    const float vsc = E4M3 && a.v_scale ? a.v_scale[hk] : 1.f;
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+        const int r = row0 + nt * 16 + r16;
+        if (r >= R) continue;
+        const float l = lacc[nt][0];
+        if (w.chunks == 1) {
+            const float inv = l > 0.f ? vsc / l : l == 0.f ? 0.f : l;
+            const int t = r / a.G, g = r - t * a.G;
+            bf16* op = a.out + (long)(w.q0 + t) * a.ldo + (long)(hk * a.G + g) * a.hd + 4 * q4;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+                if (dt * 16 < a.hd) *(bf16x4*)(op + dt * 16) = (bf16x4){f2bf(o[nt][dt][0] * inv), f2bf(o[nt][dt][1] * inv), f2bf(o[nt][dt][2] * inv), f2bf(o[nt][dt][3] * inv)};
+        } else {
+            const long pr = ((long)item * a.kv_heads + hk) * TR + wave * 32 + nt * 16 + r16;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) *(f32x4*)&a.part_o[pr * D + dt * 16 + 4 * q4] = o[nt][dt];
+            if (q4 == 0) { a.part_ml[pr * 2] = m_run[nt]; a.part_ml[pr * 2 + 1] = l; }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
 // Joins the chunks of the rows of one token and key-value head.
 // ---------------------------------------------------------------------------------------------
 template <int D, int TR>
@@ -421,7 +698,9 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a, i
     for (int g = threadIdx.x / LPR; g < a.G; g += 256 / LPR) {
         const int r = t * a.G + g, tile = r / TR;
         const Span sp = tile_span(a, w, tile, TR);
-        const int item = min(first_s + tile * w.chunks, a.grid_items - 1);           // (a cu that is no running sum: still in bounds)
+        // the tile kernel numbers a request's tiles from the last
+        const int rt = (int)(((long)w.T * a.G + TR - 1) / TR), order = TR == 128 ? max(rt - 1 - tile, 0) : tile;
+        const int item = min(first_s + order * w.chunks, a.grid_items - 1);          // (a cu that is no running sum: still in bounds)
         const int chunks = min(max(1, (sp.nb + sp.S - 1) / sp.S), a.grid_items - item);
         const long step = (long)a.kv_heads * TR, p0 = ((long)item * a.kv_heads + hk) * TR + (r - tile * TR);
         float M = -INFINITY;
@@ -443,7 +722,11 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a, i
 }
 
 // ---------------------------------------------------------------------------------------------
-static int rows_of_tile(const PagedAttnArgs* a, int max_q) { return 16; }
+// Sixteen rows a tile for a token (G rows of a key-value head), 32 for some drafted ones, 128 beyond: the matrix cores are then what counts.
+static int rows_of_tile(const PagedAttnArgs* a, int max_q) {
+    const long rows = (long)(max_q > 0 ? max_q : (a->n_tokens + a->n - 1) / (a->n > 0 ? a->n : 1)) * a->G;
+    return rows <= 16 ? 16 : rows <= 32 ? 32 : 128;
+}
 static int template_dim(const PagedAttnArgs* a) { return a->hd <= 64 ? 64 : 128; }
 
 size_t paged_partial_floats(const PagedAttnArgs* a) { return (size_t)a->grid_items * a->kv_heads * a->tile_rows * template_dim(a); }
@@ -451,7 +734,8 @@ size_t paged_partial_floats(const PagedAttnArgs* a) { return (size_t)a->grid_ite
 size_t paged_attention_plan(PagedAttnArgs* a, int n_cus, int max_q, int max_len) {
     const int TR = a->tile_rows = rows_of_tile(a, max_q);
     const long tiles = (long)a->n_tokens * a->G / TR + a->n;              // of one key-value head, at most
-    a->target = (4 * n_cus + a->kv_heads - 1) / a->kv_heads;              // four workgroups a CU
+    const int per_cu = TR == 128 ? 2 : 4;                                  // workgroups that run on a CU at once
+    a->target = (per_cu * n_cus + a->kv_heads - 1) / a->kv_heads;
     a->min_blocks = 2;                                                    // 128 keys: one block of 32 for each of the four waves
     long cap = (long)a->max_blocks << a->lps;
     if (max_len > 0 && max_len < cap) cap = max_len;
@@ -463,18 +747,23 @@ size_t paged_attention_plan(PagedAttnArgs* a, int n_cus, int max_q, int max_len)
     return (paged_partial_floats(a) + (size_t)a->grid_items * a->kv_heads * TR * 2) * sizeof(float);
 }
 
-template <int D>
-static hipError_t launch(const PagedAttnArgs* a, int e4m3, int max_q, hipStream_t st) {
+template <int D, bool E4M3, int TR>
+static hipError_t launch(const PagedAttnArgs* a, hipStream_t st) {
     const dim3 grid(a->grid_items, a->kv_heads);
-    if (e4m3) paged_attn_rows_kernel<D, true, 1><<<grid, 256, 0, st>>>(*a);
-    else paged_attn_rows_kernel<D, false, 1><<<grid, 256, 0, st>>>(*a);
+    if constexpr (TR == 128) paged_attn_tile_kernel<D, E4M3><<<grid, 256, 4 * 64 * D * sizeof(bf16), st>>>(*a);
+    else paged_attn_rows_kernel<D, E4M3, TR / 16><<<grid, 256, 0, st>>>(*a);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && a->cmax > 1) {
-        paged_attn_join_kernel<D, 16><<<dim3(a->n_tokens, a->kv_heads), 256, 0, st>>>(*a, e4m3);
+        paged_attn_join_kernel<D, TR><<<dim3(a->n_tokens, a->kv_heads), 256, 0, st>>>(*a, E4M3);
         e = hipGetLastError();
     }
     return e;
 }
-hipError_t paged_attention(const PagedAttnArgs* a, int e4m3, int max_q, hipStream_t st) {
-    return template_dim(a) == 64 ? launch<64>(a, e4m3, max_q, st) : launch<128>(a, e4m3, max_q, st);
+template <int D, bool E4M3>
+static hipError_t launch(const PagedAttnArgs* a, hipStream_t st) {
+    return a->tile_rows == 16 ? launch<D, E4M3, 16>(a, st) : a->tile_rows == 32 ? launch<D, E4M3, 32>(a, st) : launch<D, E4M3, 128>(a, st);
+}
+hipError_t paged_attention(const PagedAttnArgs* a, int e4m3, hipStream_t st) {
+    if (template_dim(a) == 64) return e4m3 ? launch<64, true>(a, st) : launch<64, false>(a, st);
+    return e4m3 ? launch<128, true>(a, st) : launch<128, false>(a, st);
 }
