@@ -173,6 +173,7 @@ extern "C" int aha_paged_attention(aha_paged* p, int layer, const void* q, int64
     a.window = window; a.scale = scale;
     a.part_o = (float*)workspace;
     a.part_ml = need ? a.part_o + paged_partial_floats(&a) : nullptr;
+    a.info = need ? (int*)(a.part_ml + (size_t)a.grid_items * a.kv_heads * a.tile_rows * 2) : nullptr;
     RUN("paged attention", paged_attention(&a, d.kv_type == AHA_KV_E4M3, (hipStream_t)st));
     return 0;
 }

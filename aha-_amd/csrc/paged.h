@@ -40,6 +40,7 @@ struct PagedAttnArgs {
     const float *k_scale, *v_scale;
     const int *table, *lens, *seqs, *cu;
     float *part_o, *part_ml;                     // [items * kv_heads][tile rows][D] / [..][2]
+    int* info;                                   // [n][2]: a request's first item and its chunks a tile
     int n, n_tokens, max_seqs, max_blocks, n_pages, lps, kv_heads, G, hd, window;
     float scale;
     int target, min_blocks, cmax;                // the split: see schedule() in paged_attention.hip
@@ -51,5 +52,5 @@ hipError_t paged_truncate(const PagedReserveArgs* a, hipStream_t st);
 hipError_t paged_append(const PagedAppendArgs* a, hipStream_t st);
 // fills target / min_blocks / cmax / grid_items for max_len keys at most and returns the bytes of partial results the call needs (0: no split)
 size_t paged_attention_plan(PagedAttnArgs* a, int n_cus, int max_q, int max_len);
-size_t paged_partial_floats(const PagedAttnArgs* a);          // floats of part_o; part_ml lies behind them
+size_t paged_partial_floats(const PagedAttnArgs* a);          // floats of part_o; part_ml and info lie behind them
 hipError_t paged_attention(const PagedAttnArgs* a, int e4m3, hipStream_t st);

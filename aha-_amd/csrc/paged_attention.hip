@@ -24,7 +24,7 @@ typedef const __attribute__((address_space(4))) int* table_t;         // read by
 // into C_i = clamp(floor(nb_i / S), 1, cmax) chunks of equal length: W / target + (number of tiles) items at most, whatever the lengths are,
 // and no item longer than 2 S.  Items are numbered request by request, tile by tile.
 // ---------------------------------------------------------------------------------------------
-struct Work { int req, seq, q0, T, L, tile, chunk, chunks; };
+struct Work { int req, seq, q0, T, L, first, tile, chunk, chunks; };
 
 static __device__ __forceinline__ void request_shape(const PagedAttnArgs& a, int i, int* seq, int* q0, int* T, int* L) {
     *seq = a.seqs[i];
@@ -44,8 +44,8 @@ static __device__ __forceinline__ void request_tiles(const PagedAttnArgs& a, int
     if (a.window) keys = (int)min((long)keys, (long)a.window + TR / a.G + 65);
     *nb = (keys + 63) >> 6;
 }
-template <int NTH, int TR, class Want>
-static __device__ __forceinline__ bool schedule(const PagedAttnArgs& a, Want want, Work* out) {
+template <int NTH, int TR>
+static __device__ __forceinline__ bool schedule(const PagedAttnArgs& a, int item, Work* out) {
     __shared__ float fsum[NTH / 64];
     __shared__ int isum[NTH / 64];
     __shared__ Work found;
@@ -83,15 +83,22 @@ static __device__ __forceinline__ bool schedule(const PagedAttnArgs& a, Want wan
         __syncthreads();
         int before = base;
         for (int k = 0; k < NTH / 64; ++k) { if (k < wave) before += isum[k]; base += isum[k]; }
-        if (i0 + tid < a.n) {
-            Work f = {i0 + tid, seq, q0, T, L, 0, 0, C};
-            if (want(before + x - items, items, &f)) { found = f; have = 1; }
+        const int k = item - (before + x - items);
+        if (k >= 0 && k < items) {
+            found = {i0 + tid, seq, q0, T, L, item - k, k / C, k % C, C};
+            have = 1;
         }
         __syncthreads();
         if (have) break;
     }
     if (!have) return false;
-    *out = found;
+    const Work f = found;                                   // the same in all: scalars
+    out->req = __builtin_amdgcn_readfirstlane(f.req); out->seq = __builtin_amdgcn_readfirstlane(f.seq);
+    out->q0 = __builtin_amdgcn_readfirstlane(f.q0); out->T = __builtin_amdgcn_readfirstlane(f.T); out->L = __builtin_amdgcn_readfirstlane(f.L);
+    out->first = __builtin_amdgcn_readfirstlane(f.first); out->tile = __builtin_amdgcn_readfirstlane(f.tile);
+    out->chunk = __builtin_amdgcn_readfirstlane(f.chunk); out->chunks = __builtin_amdgcn_readfirstlane(f.chunks);
+    // for the join: where a request's partial results are
+    if (item == out->first && blockIdx.y == 0 && tid == 0 && a.cmax > 1) { a.info[2 * out->req] = out->first; a.info[2 * out->req + 1] = out->chunks; }
     return true;
 }
 
@@ -108,6 +115,14 @@ static __device__ __forceinline__ Span tile_span(const PagedAttnArgs& a, const W
     return s;
 }
 
+// a chunk without keys says so to the join, which then leaves its partial output alone
+template <int TR>
+static __device__ __forceinline__ void no_keys(const PagedAttnArgs& a, int item, int hk) {
+    for (int r = threadIdx.x; r < TR; r += blockDim.x) {
+        float* ml = a.part_ml + (((long)item * a.kv_heads + hk) * TR + r) * 2;
+        ml[0] = -INFINITY; ml[1] = 0.f;
+    }
+}
 static __device__ __forceinline__ bool nonfinite(bf16x8 v) {
     const u32x4 u = __builtin_bit_cast(u32x4, v);
     bool bad = false;
@@ -139,21 +154,12 @@ __global__ __launch_bounds__(256) void paged_attn_rows_kernel(PagedAttnArgs a) {
 
     const int item = blockIdx.x, hk = blockIdx.y;
     Work w;
-    if (!schedule<256, TR>(a, [&](int first, int items, Work* f) {
-            const int k = item - first;
-            if (k < 0 || k >= items) return false;
-            f->tile = k / f->chunks; f->chunk = k - f->tile * f->chunks;
-            return true;
-        }, &w)) return;
+    if (!schedule<256, TR>(a, item, &w)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int q4 = lane >> 4, r16 = lane & 15;
-    w.seq = __builtin_amdgcn_readfirstlane(w.seq); w.q0 = __builtin_amdgcn_readfirstlane(w.q0);
-    w.T = __builtin_amdgcn_readfirstlane(w.T); w.L = __builtin_amdgcn_readfirstlane(w.L);
-    w.tile = __builtin_amdgcn_readfirstlane(w.tile); w.chunk = __builtin_amdgcn_readfirstlane(w.chunk);
-    w.chunks = __builtin_amdgcn_readfirstlane(w.chunks);
     const Span sp = tile_span(a, w, w.tile, TR);
     const int b0 = w.chunk * sp.S, b1 = min(sp.nb, b0 + sp.S);
-    if (b0 >= b1 && w.chunk) return;                       // a chunk without keys; chunk 0 writes the zeros of rows that see nothing
+    if (b0 >= b1 && w.chunks > 1) { no_keys<TR>(a, item, hk); return; }
     const int R = w.T * a.G, base_pos = w.L - w.T;
 
     // rows of this lane (one a tile) and their queries
@@ -429,22 +435,13 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
 
     const int item = blockIdx.x, hk = blockIdx.y;
     Work w;
-    if (!schedule<256, TR>(a, [&](int first, int items, Work* f) {
-            const int k = item - first;
-            if (k < 0 || k >= items) return false;
-            f->tile = items / f->chunks - 1 - k / f->chunks;              // the longest rows of a prompt first
-            f->chunk = k % f->chunks;
-            return true;
-        }, &w)) return;
+    if (!schedule<256, TR>(a, item, &w)) return;
+    w.tile = (int)(((long)w.T * a.G + TR - 1) / TR) - 1 - w.tile;         // the longest rows of a prompt first
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int q4 = lane >> 4, r16 = lane & 15;
-    w.seq = __builtin_amdgcn_readfirstlane(w.seq); w.q0 = __builtin_amdgcn_readfirstlane(w.q0);
-    w.T = __builtin_amdgcn_readfirstlane(w.T); w.L = __builtin_amdgcn_readfirstlane(w.L);
-    w.tile = __builtin_amdgcn_readfirstlane(w.tile); w.chunk = __builtin_amdgcn_readfirstlane(w.chunk);
-    w.chunks = __builtin_amdgcn_readfirstlane(w.chunks);
     const Span sp = tile_span(a, w, w.tile, TR);
     const int b0 = w.chunk * sp.S, b1 = min(sp.nb, b0 + sp.S);
-    if (b0 >= b1 && w.chunk) return;
+    if (b0 >= b1 && w.chunks > 1) { no_keys<TR>(a, item, hk); return; }
     const int R = w.T * a.G, base_pos = w.L - w.T;
     const int row0 = w.tile * TR + wave * 32;
     const bool wave_on = row0 < R;
@@ -680,47 +677,67 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
 }
 
 // ---------------------------------------------------------------------------------------------
-// Joins the chunks of the rows of one token and key-value head.
+// Joins the chunks of split rows, a wave for each token and query head (or, of many tokens, for each token: most then have nothing to join).
+// A lane knows one chunk's maximum and sum, so the weights of 64 chunks take one load; then 64 / (D / 4) partial rows are added at a time.  What
+// bounds it is the chain request -> item -> maximum -> output: the request is found by counting, not by bisection.
 // ---------------------------------------------------------------------------------------------
 template <int D, int TR>
-__global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a, int e4m3) {
-    const int tok = blockIdx.x, hk = blockIdx.y;
-    __shared__ int first_s;
-    Work w;
-    if (!schedule<256, TR>(a, [&](int first, int items, Work* f) {
-            if (items == 0 || tok < f->q0 || tok >= f->q0 + f->T) return false;
-            first_s = first;
-            return true;
-        }, &w)) return;
-    if (w.chunks == 1) return;
-    const int t = max(tok - w.q0, 0), LPR = D / 4, lane = threadIdx.x % LPR;
-    const float vsc = e4m3 && a.v_scale ? a.v_scale[hk] : 1.f;
-    for (int g = threadIdx.x / LPR; g < a.G; g += 256 / LPR) {
-        const int r = t * a.G + g, tile = r / TR;
-        const Span sp = tile_span(a, w, tile, TR);
-        // the tile kernel numbers a request's tiles from the last
-        const int rt = (int)(((long)w.T * a.G + TR - 1) / TR), order = TR == 128 ? max(rt - 1 - tile, 0) : tile;
-        const int item = min(first_s + order * w.chunks, a.grid_items - 1);          // (a cu that is no running sum: still in bounds)
-        const int chunks = min(max(1, (sp.nb + sp.S - 1) / sp.S), a.grid_items - item);
-        const long step = (long)a.kv_heads * TR, p0 = ((long)item * a.kv_heads + hk) * TR + (r - tile * TR);
-        float M = -INFINITY;
-        for (int c = 0; c < chunks; ++c) M = fmaxf(M, a.part_ml[(p0 + c * step) * 2]);
-        const float ref = M == -INFINITY ? 0.f : M;
-        float l = 0.f;
+__global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a, int e4m3, int heads_each) {
+    constexpr int LPR = D / 4, AT = 64 / LPR;               // lanes of a row, rows at a time
+    const int heads = a.kv_heads * a.G, groups = heads / heads_each;
+    const int unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
+    const int tok = unit / groups;
+    if (tok >= a.n_tokens) return;
+    int req = 0;
+    if (a.n <= 512) {
+#pragma unroll 4
+        for (int i0 = 0; i0 < a.n; i0 += 64) req += __popcll(__ballot(i0 + lane < a.n && a.cu[min(i0 + lane, a.n - 1) + 1] <= tok));
+    } else {
+        int hi = a.n;
+        while (req < hi) { const int mid = (req + hi) >> 1; if (a.cu[mid + 1] <= tok) req = mid + 1; else hi = mid; }
+    }
+    if (req >= a.n) return;                                 // behind the last request
+    const int q0 = a.cu[req], T = a.cu[req + 1] - q0, seq = a.seqs[req], first = a.info[2 * req], chunks = a.info[2 * req + 1];
+    if (tok < q0 || (unsigned)seq >= (unsigned)a.max_seqs || chunks <= 1) return;
+    const int rt = (int)(((long)T * a.G + TR - 1) / TR), col = lane % LPR * 4, sub = lane / LPR;
+    for (int h = unit % groups * heads_each, end = h + heads_each; h < end; ++h) {
+        const int hk = h / a.G, r = (tok - q0) * a.G + h - hk * a.G, tile = r / TR;
+        const long item = first + (long)(TR == 128 ? rt - 1 - tile : tile) * chunks;
+        if (item < 0 || item + chunks > a.grid_items) return;             // (a cu that is no running sum)
+        const long step = (long)a.kv_heads * TR, p0 = (item * a.kv_heads + hk) * TR + (r - tile * TR);
+        float M = -INFINITY, l = 0.f;
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-        for (int c = 0; c < chunks; ++c) {
-            const float f = __builtin_amdgcn_exp2f(a.part_ml[(p0 + c * step) * 2] - ref);
-            l += a.part_ml[(p0 + c * step) * 2 + 1] * f;
-            const f32x4 v = *(const f32x4*)&a.part_o[(p0 + c * step) * D + lane * 4];
+        for (int c0 = 0; c0 < chunks; c0 += 64) {
+            float m = -INFINITY, ls = 0.f;
+            if (c0 + lane < chunks) { const float2 x = *(const float2*)&a.part_ml[(p0 + (c0 + lane) * step) * 2]; m = x.x; ls = x.y; }
+            const float Mn = fmaxf(M, wave_max(m)), ref = Mn == -INFINITY ? 0.f : Mn;
+            const float f = __builtin_amdgcn_exp2f(m - ref), old = __builtin_amdgcn_exp2f(M - ref);
+            l = l * old + wave_sum(ls * f);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] += v[e] * f;
+            for (int e = 0; e < 4; ++e) acc[e] *= old;
+            M = Mn;
+            const int cn = min(64, chunks - c0);
+#pragma unroll 4
+            for (int c = 0; c < cn; c += AT) {
+                const float fc = __shfl(f, min(c + sub, 63), 64), mc = __shfl(m, min(c + sub, 63), 64);
+                if (c + sub < cn && mc != -INFINITY) {
+                    const f32x4 v = *(const f32x4*)&a.part_o[(p0 + (c0 + c + sub) * step) * D + col];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[e] += v[e] * fc;
+                }
+            }
         }
-        const float inv = l > 0.f ? vsc / l : l == 0.f ? 0.f : l;
-        bf16x4 ov = {f2bf(acc[0] * inv), f2bf(acc[1] * inv), f2bf(acc[2] * inv), f2bf(acc[3] * inv)};
-        if (lane * 4 < a.hd) *(bf16x4*)(a.out + (long)tok * a.ldo + (long)(hk * a.G + g) * a.hd + lane * 4) = ov;
+#pragma unroll
+        for (int o = LPR; o < 64; o <<= 1)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], o, 64);
+        const float inv = l > 0.f ? (e4m3 && a.v_scale ? a.v_scale[hk] : 1.f) / l : l == 0.f ? 0.f : l;
+        if (sub == 0 && col < a.hd)
+            *(bf16x4*)(a.out + (long)tok * a.ldo + (long)h * a.hd + col) = (bf16x4){f2bf(acc[0] * inv), f2bf(acc[1] * inv), f2bf(acc[2] * inv), f2bf(acc[3] * inv)};
     }
 }
 
+// ---------------------------------------------------------------------------------------------
 // ---------------------------------------------------------------------------------------------
 // Sixteen rows a tile for a token (G rows of a key-value head), 32 for some drafted ones, 128 beyond: the matrix cores are then what counts.
 static int rows_of_tile(const PagedAttnArgs* a, int max_q) {
@@ -744,7 +761,7 @@ size_t paged_attention_plan(PagedAttnArgs* a, int n_cus, int max_q, int max_len)
     const long by_split = a->target + a->target / 1024 + 8 + tiles, by_len = tiles * a->cmax;
     a->grid_items = (int)(by_len < by_split ? by_len : by_split);
     if (a->cmax == 1) return 0;
-    return (paged_partial_floats(a) + (size_t)a->grid_items * a->kv_heads * TR * 2) * sizeof(float);
+    return (paged_partial_floats(a) + (size_t)a->grid_items * a->kv_heads * TR * 2) * sizeof(float) + (size_t)a->n * 2 * sizeof(int);
 }
 
 template <int D, bool E4M3, int TR>
@@ -754,7 +771,8 @@ static hipError_t launch(const PagedAttnArgs* a, hipStream_t st) {
     else paged_attn_rows_kernel<D, E4M3, TR / 16><<<grid, 256, 0, st>>>(*a);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && a->cmax > 1) {
-        paged_attn_join_kernel<D, TR><<<dim3(a->n_tokens, a->kv_heads), 256, 0, st>>>(*a, E4M3);
+        const int heads = a->kv_heads * a->G, each = a->n_tokens >= 2048 ? heads : 1;
+        paged_attn_join_kernel<D, TR><<<(int)(((long)a->n_tokens * (heads / each) + 3) / 4), 256, 0, st>>>(*a, E4M3, each);
         e = hipGetLastError();
     }
     return e;

@@ -90,27 +90,29 @@ class PagedKVCache:
             raise ValueError(f"{name}: a contiguous {dtype} tensor {list(shape)} on {self.device} is needed, not {t.dtype} {list(t.shape)} on {t.device}")
         return t
 
+    # (these run on every call of a layer: one test of what is right, the reasons only where it is not)
     def _ints(self, name, t, n=None):
-        if t.dtype != torch.int32 or t.device != self.device or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.shape[0] != n):
-            raise ValueError(f"{name}: a contiguous int32 tensor{'' if n is None else f' of {n} elements'} on {self.device} is needed, not {t.dtype} {list(t.shape)} on {t.device}")
-        return t.data_ptr()
+        if t.dtype is torch.int32 and t.device == self.device and t.dim() == 1 and (n is None or t.shape[0] == n) and t.is_contiguous():
+            return t.data_ptr()
+        raise ValueError(f"{name}: a contiguous int32 tensor{'' if n is None else f' of {n} elements'} on {self.device} is needed, not {t.dtype} {list(t.shape)} on {t.device}")
 
     def _rows(self, name, x, heads=None, out=False):
         """[N, heads, head_dim] or [N, heads * head_dim] -> (tensor, heads, row stride); rows may be strided, their elements not."""
-        D = self.head_dim
-        if x.dtype != torch.bfloat16 or x.device != self.device or x.dim() not in (2, 3) or (x.dim() == 3 and x.shape[2] != D) or (x.dim() == 2 and x.shape[1] % D):
+        D, shape, stride = self.head_dim, x.shape, x.stride()
+        if x.dtype is not torch.bfloat16 or x.device != self.device or len(shape) not in (2, 3) or (shape[2] != D if len(shape) == 3 else shape[1] % D):
             raise ValueError(f"{name}: a bfloat16 tensor [N, heads, {D}] or [N, heads * {D}] on {self.device} is needed, not {x.dtype} {list(x.shape)} on {x.device}")
-        h = x.shape[1] if x.dim() == 3 else x.shape[1] // D
+        h = shape[1] if len(shape) == 3 else shape[1] // D
         if heads is not None and h != heads:
             raise ValueError(f"{name}: {heads} heads are needed, not {h}")
-        if x.stride(-1) != 1 or (x.dim() == 3 and h > 1 and x.stride(1) != D) or (x.shape[0] > 1 and x.stride(0) < h * D):
+        many = shape[0] > 1
+        if stride[-1] != 1 or (len(shape) == 3 and h > 1 and stride[1] != D) or (many and stride[0] < h * D):
             if out:
                 raise ValueError(f"{name}: the heads of a row must be contiguous and rows must not overlap")
-            x = x.contiguous()
-        return x, h, x.stride(0) if x.shape[0] > 1 else h * D
+            return x.contiguous(), h, h * D
+        return x, h, stride[0] if many else h * D
 
     def _stream(self) -> int:
-        return torch.cuda.current_stream(self.device).cuda_stream
+        return torch._C._cuda_getCurrentRawStream(self.device.index)
 
     def _chk(self, rc: int):
         if rc != 0:
@@ -141,17 +143,16 @@ class PagedKVCache:
         if n_tokens < 0:
             raise ValueError("n_tokens must not be negative")
         sp, cp = self._ints("seqs", seqs), self._ints("counts", counts, n)
-        out = torch.empty((2 * n_tokens + n + 3,), dtype=torch.int32, device=self.device)
-        slots, positions, cu, status = out.split((n_tokens, n_tokens, n + 1, 2))
+        out = torch.empty(2 * n_tokens + n + 3, dtype=torch.int32, device=self.device)
         p = out.data_ptr()
         self._chk(self.lib.aha_paged_reserve(self.handle, sp, cp, n, p, p + 4 * n_tokens, n_tokens, p + 8 * n_tokens, p + 8 * n_tokens + 4 * (n + 1), self._stream()))
-        return slots, positions, cu, status
+        return out.split_with_sizes((n_tokens, n_tokens, n + 1, 2))
 
     def truncate(self, seqs: torch.Tensor, lens: torch.Tensor) -> torch.Tensor:
         """Sequences are cut to `lens` tokens (0 releases them) -> status [2]."""
         n = seqs.shape[0]
         sp, lp = self._ints("seqs", seqs), self._ints("lens", lens, n)
-        status = torch.empty((2,), dtype=torch.int32, device=self.device)
+        status = torch.empty(2, dtype=torch.int32, device=self.device)
         self._chk(self.lib.aha_paged_truncate(self.handle, sp, lp, n, status.data_ptr(), self._stream()))
         return status
 
@@ -171,12 +172,11 @@ class PagedKVCache:
         pp = self._ints("positions", positions, n) if cos is not None else None
         heads, ldq, ldo, qp, op = 0, 0, 0, None, None
         if q is not None:
+            q, heads, ldq = self._rows("q", q)
             if q_out is None:
-                q, heads, ldq = self._rows("q", q)
-                q_out = torch.empty((n, heads, self.head_dim), dtype=torch.bfloat16, device=self.device)
+                q_out = torch.empty(n, heads, self.head_dim, dtype=torch.bfloat16, device=self.device)
                 ldo = heads * self.head_dim
             else:
-                q, heads, ldq = self._rows("q", q)
                 q_out, _, ldo = self._rows("q_out", q_out, heads, out=True)
                 if q_out.shape[0] != n:
                     raise ValueError("q_out needs as many tokens as q")
@@ -194,20 +194,20 @@ class PagedKVCache:
         n, N = seqs.shape[0], q.shape[0]
         sp, cp = self._ints("seqs", seqs), self._ints("cu", cu, n + 1)
         if out is None:
-            out, ldo = torch.empty((N, heads, self.head_dim), dtype=torch.bfloat16, device=self.device), heads * self.head_dim
+            out, ldo = torch.empty(N, heads, self.head_dim, dtype=torch.bfloat16, device=self.device), heads * self.head_dim
         else:
             out, _, ldo = self._rows("out", out, heads, out=True)
             if out.shape[0] != N:
                 raise ValueError("out needs as many tokens as q")
         key = (heads, N, n, max_q, max_len)
         need = self._workspace.get(key)
-        if need is None:
+        if need is None:                                           # (a function of the sizes alone, asked for once)
             b = C.c_size_t()
             self._chk(self.lib.aha_paged_attention_workspace(self.handle, heads, N, n, max_q, max_len, C.byref(b)))
             if len(self._workspace) >= 4096:
                 self._workspace.clear()
             need = self._workspace[key] = b.value
-        ws = torch.empty((need,), dtype=torch.uint8, device=self.device) if need else None
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
         self._chk(self.lib.aha_paged_attention(self.handle, layer, q.data_ptr(), ldq, heads, sp, cp, n, N, max_q, max_len, window,
                                                self.head_dim ** -0.5 if scale is None else scale, out.data_ptr(), ldo, ws.data_ptr() if need else None, need, self._stream()))
         return out
