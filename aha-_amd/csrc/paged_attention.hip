@@ -98,7 +98,7 @@ static __device__ __forceinline__ bool schedule(const PagedAttnArgs& a, int item
     out->first = __builtin_amdgcn_readfirstlane(f.first); out->tile = __builtin_amdgcn_readfirstlane(f.tile);
     out->chunk = __builtin_amdgcn_readfirstlane(f.chunk); out->chunks = __builtin_amdgcn_readfirstlane(f.chunks);
     // for the join: where a request's partial results are
-    if (item == out->first && blockIdx.y == 0 && tid == 0 && a.cmax > 1) { a.info[2 * out->req] = out->first; a.info[2 * out->req + 1] = out->chunks; }
+    if (item == out->first && (int)blockIdx.x == item * a.kv_heads && tid == 0 && a.cmax > 1) { a.info[2 * out->req] = out->first; a.info[2 * out->req + 1] = out->chunks; }
     return true;
 }
 
@@ -152,7 +152,7 @@ __global__ __launch_bounds__(256) void paged_attn_rows_kernel(PagedAttnArgs a) {
     __shared__ __attribute__((aligned(16))) bf16 Vs[4][32 * VST];
     __shared__ float sm[4][16], sl[4][16];
 
-    const int item = blockIdx.x, hk = blockIdx.y;
+    const int item = blockIdx.x / a.kv_heads, hk = blockIdx.x - item * a.kv_heads;
     Work w;
     if (!schedule<256, TR>(a, item, &w)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -412,7 +412,7 @@ __global__ __launch_bounds__(256) void paged_attn_rows_kernel(PagedAttnArgs a) {
 // ---------------------------------------------------------------------------------------------
 // Many rows (frames, prompts): bound by the matrix cores and the exponentials.  A workgroup's four waves have 32 rows each and share blocks of
 // 64 keys, K and V double-buffered in LDS: the next block is under way while this one is computed, with one barrier a block.  bf16 pages go
-// straight to LDS (global_load_lds, 1 KiB of contiguous rows an instruction), e4m3 through registers, where they become bf16.  In LDS a row's
+// straight to LDS (buffer_load ... lds, 1 KiB of contiguous rows an instruction), e4m3 through registers, where they become bf16.  In LDS a row's
 // 16-byte chunks are permuted by its number: sixteen rows read at one column, or eight rows at two, touch every bank once.
 // P is rounded to bf16 (half a step, 2^-8 of p, as the output itself is); the sum of the row is taken from the rounded values, by the matrix cores
 // (a product with ones), so that numerator and denominator round alike.  The running maximum moves only when a score exceeds it by 2^8: until
@@ -423,8 +423,12 @@ template <int D> struct TileLds {
     static __device__ __forceinline__ int k_slot(int row, int ch) { return row * D + ((ch ^ (D == 128 ? row & 15 : (row >> 1) & 7)) << 3); }
     static __device__ __forceinline__ int v_slot(int row, int ch) { return row * D + ((ch ^ (D == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3))) << 3); }
 };
-typedef const __attribute__((address_space(1))) unsigned* gptr_t;
-typedef __attribute__((address_space(3))) unsigned* lptr_t;
+// sixteen bytes a lane, from its offset in `from` to lane * 16 behind `lds`
+static __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t from, bf16* lds, unsigned off) {
+#ifdef __HIP_DEVICE_COMPILE__
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)lds, 16, off, 0, 0, 0);
+#endif
+}
 
 template <int D, bool E4M3>
 __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a) {
@@ -433,7 +437,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
     extern __shared__ __attribute__((aligned(16))) bf16 kv[];             // [buffer][K, V][64][D]
     __shared__ int odd_s[2];
 
-    const int item = blockIdx.x, hk = blockIdx.y;
+    const int item = blockIdx.x / a.kv_heads, hk = blockIdx.x - item * a.kv_heads;
     Work w;
     if (!schedule<256, TR>(a, item, &w)) return;
     w.tile = (int)(((long)w.T * a.G + TR - 1) / TR) - 1 - w.tile;         // the longest rows of a prompt first
@@ -488,24 +492,31 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
     auto no_page = [&](int page) { return (unsigned)page >= (unsigned)a.n_pages; };
     constexpr int NL = E4M3 ? D / 64 : D / 32;              // 16-byte loads a lane of sixteen rows
     u32x4 kreg[NL], vreg[NL];
-    auto stage = [&](int key0, int page, int buf) {         // wave w has keys 16 w .. 16 w + 15 of a block; bf16: into LDS; e4m3: into registers
-        page = no_page(page) ? 0 : page;
-        const long off = page * page_bytes + (long)((key0 + wave * 16) & P1) * row_bytes;
+    // a lane's byte offsets within sixteen rows: in LDS a row's chunk c lies in place c ^ f(row), so the lane of that place asks for it
+    unsigned koff[NL], voff[NL];
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
         if constexpr (!E4M3) {
-#pragma unroll
-            for (int i = 0; i < NL; ++i) {
-                const int row = i * LD::RPP + lane / LD::CPR, c = lane % LD::CPR, rb = wave * 16 + row;
-                const int ck = (LD::k_slot(rb, c) - rb * D) * 2, cv = (LD::v_slot(rb, c) - rb * D) * 2;        // the chunk that belongs in this place
-                __builtin_amdgcn_global_load_lds((gptr_t)(kp + off + row * row_bytes + min(ck, row_bytes - 16)), (lptr_t)(kv + buf * 2 * BLK + (wave * 16 + i * LD::RPP) * D), 16, 0, 0);
-                __builtin_amdgcn_global_load_lds((gptr_t)(vp + off + row * row_bytes + min(cv, row_bytes - 16)), (lptr_t)(kv + buf * 2 * BLK + BLK + (wave * 16 + i * LD::RPP) * D), 16, 0, 0);
-            }
+            const int row = i * LD::RPP + lane / LD::CPR, c = lane % LD::CPR;
+            koff[i] = row * row_bytes + min((LD::k_slot(row, c) - row * D) * 2, row_bytes - 16);
+            voff[i] = row * row_bytes + min((LD::v_slot(row, c) - row * D) * 2, row_bytes - 16);
         } else {
-            constexpr int C = D / 16;
+            const int idx = i * 64 + lane;
+            koff[i] = voff[i] = idx / (D / 16) * row_bytes + min(idx % (D / 16) * 16, row_bytes - 16);
+        }
+    }
+    auto stage = [&](int key0, int page, int buf) {         // wave w has keys 16 w .. 16 w + 15 of a block; bf16: into LDS; e4m3: into registers
+        const long off = (no_page(page) ? 0 : page) * page_bytes + (long)((key0 + wave * 16) & P1) * row_bytes;
+        const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void*)(kp + off), 0, 16 * row_bytes, 0x00020000);
+        const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void*)(vp + off), 0, 16 * row_bytes, 0x00020000);
 #pragma unroll
-            for (int i = 0; i < NL; ++i) {
-                const int idx = i * 64 + lane, row = idx / C, cb = min(idx % C * 16, row_bytes - 16);
-                kreg[i] = *(const u32x4*)(kp + off + row * row_bytes + cb);
-                vreg[i] = *(const u32x4*)(vp + off + row * row_bytes + cb);
+        for (int i = 0; i < NL; ++i) {
+            if constexpr (!E4M3) {
+                load_to_lds(kr, kv + buf * 2 * BLK + (wave * 16 + i * LD::RPP) * D, koff[i]);
+                load_to_lds(vr, kv + buf * 2 * BLK + BLK + (wave * 16 + i * LD::RPP) * D, voff[i]);
+            } else {
+                kreg[i] = __builtin_amdgcn_raw_buffer_load_b128(kr, koff[i], 0, 0);
+                vreg[i] = __builtin_amdgcn_raw_buffer_load_b128(vr, voff[i], 0, 0);
             }
         }
     };
@@ -527,8 +538,14 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
 
     int buf = 0;
     // the wave's own page a block ahead; all four of the block itself, for the mask
+    const bool one_page = a.lps >= 6;                       // a block lies in one page
     int mine = look_up(sp.first + b0 * 64, wave);
-    int p0 = look_up(sp.first + b0 * 64, 0), p1 = look_up(sp.first + b0 * 64, 1), p2 = look_up(sp.first + b0 * 64, 2), p3 = look_up(sp.first + b0 * 64, 3);
+    int p0, p1, p2, p3;
+    auto look_up_all = [&](int key0) {
+        p0 = p1 = p2 = p3 = look_up(key0, 0);
+        if (!one_page) { p1 = look_up(key0, 1); p2 = look_up(key0, 2); p3 = look_up(key0, 3); }
+    };
+    look_up_all(sp.first + b0 * 64);
     if (b0 < b1) { stage(sp.first + b0 * 64, mine, 0); unstage(0); }
     mine = look_up(sp.first + b0 * 64 + 64, wave);
     for (int b = b0; b < b1; ++b, buf ^= 1) {
@@ -556,7 +573,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
         if (b + 1 < b1) {
             stage(key0 + 64, mine, buf ^ 1);
             mine = look_up(key0 + 128, wave);
-            p0 = look_up(key0 + 64, 0); p1 = look_up(key0 + 64, 1); p2 = look_up(key0 + 64, 2); p3 = look_up(key0 + 64, 3);
+            look_up_all(key0 + 64);
         }
         // a wave whose rows see nothing of the block, or that has none, only keeps the barriers
         if (wave_on && key0 <= wpos_hi && (!a.window || key0 + 63 > wpos_lo - a.window)) {
@@ -573,28 +590,46 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
                     s[1][kt] = mfma16(kf, qf[1][ks], s[1][kt]);
                 }
             }
-            const bool masked = !plain && (bad || key0 + 63 > wpos_lo || (a.window && key0 <= wpos_hi - a.window));
-            bf16x8 pb[2][2];
+            if (!plain && (bad || key0 + 63 > wpos_lo || (a.window && key0 <= wpos_hi - a.window))) {
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt) {
-                if (masked) {
+                for (int nt = 0; nt < 2; ++nt) {
+                    int ahead = pos[nt] - key0 - 4 * q4;    // the last key the row sees, from this lane's first
+                    asm volatile("" : "+v"(ahead));         // (computed here, not kept in registers through the loop)
+                    const int least = a.window ? ahead - a.window : -0x40000000;
 #pragma unroll
                     for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const int j = key0 + kt * 16 + 4 * q4 + e;
-                            const bool see = j <= pos[nt] && !(bad >> kt & 1) && (!a.window || j > pos[nt] - a.window);
+                            const bool see = kt * 16 + e <= ahead && kt * 16 + e > least && !(bad >> kt & 1);
                             s[nt][kt][e] = see ? s[nt][kt][e] : -INFINITY;
                         }
                 }
-                float mx = fmaxf(fmaxf(s[nt][0][0], s[nt][0][1]), fmaxf(s[nt][0][2], s[nt][0][3]));
+            }
+            bf16x8 pb[2][2];
 #pragma unroll
-                for (int kt = 1; kt < 4; ++kt) mx = fmaxf(mx, fmaxf(fmaxf(s[nt][kt][0], s[nt][kt][1]), fmaxf(s[nt][kt][2], s[nt][kt][3])));
-                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-                mx *= c2;
-                if (__any(mx > m_run[nt] + 8.f)) {          // (-inf + 8 = -inf: the first key a row sees sets its reference)
-                    const float m_new = mx > m_run[nt] + 8.f ? mx : m_run[nt];
+            for (int nt = 0; nt < 2; ++nt) {
+                // exponentials against the running reference; only where one of them exceeds 2^8, or a row has no reference yet, is the
+                // row's maximum looked for
+                float p[4][4], top = 0.f;
+                auto exps = [&]() {
+                    const float ref = m_run[nt] == -INFINITY ? 0.f : -m_run[nt];
+                    top = 0.f;
+#pragma unroll
+                    for (int kt = 0; kt < 4; ++kt) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) p[kt][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nt][kt][e], c2, ref));
+                        top = fmaxf(fmaxf(top, p[kt][0]), fmaxf(p[kt][1], fmaxf(p[kt][2], p[kt][3])));
+                    }
+                };
+                exps();
+                if (__any(top > 256.f || m_run[nt] == -INFINITY)) {
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int kt = 0; kt < 4; ++kt) mx = fmaxf(mx, fmaxf(fmaxf(s[nt][kt][0], s[nt][kt][1]), fmaxf(s[nt][kt][2], s[nt][kt][3])));
+                    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+                    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                    mx *= c2;
+                    const float m_new = mx > m_run[nt] + 8.f ? mx : m_run[nt];        // (-inf + 8 = -inf: the first key a row sees)
                     const float alpha = m_new == m_run[nt] ? 1.f : __builtin_amdgcn_exp2f(m_run[nt] - m_new);
                     m_run[nt] = m_new;
 #pragma unroll
@@ -603,13 +638,12 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
                     for (int i = 0; i < DT; ++i)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) o[nt][i][e] *= alpha;
+                    exps();
                 }
-                const float ref = m_run[nt] == -INFINITY ? 0.f : -m_run[nt];
 #pragma unroll
                 for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        pb[nt][kt >> 1][(kt & 1) * 4 + e] = f2bf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[nt][kt][e], c2, ref)));
+                    for (int e = 0; e < 4; ++e) pb[nt][kt >> 1][(kt & 1) * 4 + e] = f2bf(p[kt][e]);
 #pragma unroll
                 for (int kp_ = 0; kp_ < 2; ++kp_) lacc[nt] = mfma16(ones, pb[nt][kp_], lacc[nt]);
             }
@@ -631,6 +665,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
                     }
             } else {
                 for (int p = wpos_lo; p <= wpos_hi; ++p) {  // each position's rows on their own, with the keys they see (0 * inf is no zero)
+                    int ahead = p - key0 - 4 * q4;
+                    asm volatile("" : "+v"(ahead));
+                    const int least = a.window ? ahead - a.window : -0x40000000;
 #pragma unroll
                     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -638,8 +675,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
                             bf16x8 vf = v_frag(dt, kp_);
 #pragma unroll
                             for (int e = 0; e < 8; ++e) {
-                                const int j = key0 + kp_ * 32 + (e >> 2) * 16 + 4 * q4 + (e & 3);
-                                if (j > p || (a.window && j <= p - a.window)) vf[e] = 0;
+                                const int j = kp_ * 32 + (e >> 2) * 16 + (e & 3);
+                                if (j > ahead || j <= least) vf[e] = 0;
                             }
 #pragma unroll
                             for (int nt = 0; nt < 2; ++nt) {
@@ -766,7 +803,7 @@ size_t paged_attention_plan(PagedAttnArgs* a, int n_cus, int max_q, int max_len)
 
 template <int D, bool E4M3, int TR>
 static hipError_t launch(const PagedAttnArgs* a, hipStream_t st) {
-    const dim3 grid(a->grid_items, a->kv_heads);
+    const int grid = a->grid_items * a->kv_heads;
     if constexpr (TR == 128) paged_attn_tile_kernel<D, E4M3><<<grid, 256, 4 * 64 * D * sizeof(bf16), st>>>(*a);
     else paged_attn_rows_kernel<D, E4M3, TR / 16><<<grid, 256, 0, st>>>(*a);
     hipError_t e = hipGetLastError();
