@@ -19,10 +19,11 @@ typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
 typedef const __attribute__((address_space(4))) int* table_t;         // read by scalar loads: nothing writes the tables while a call runs
 
 // ---------------------------------------------------------------------------------------------
-// The split.  Request i: R_i = G * T_i rows in rt_i tiles of TR, at most nb_i blocks of 64 keys a tile.  With W = sum rt_i * nb_i blocks of
-// work in all and `target` workgroups wanted, a chunk is at least S = max(min_blocks, W / target) blocks long and a tile of request i is cut
-// into C_i = clamp(floor(nb_i / S), 1, cmax) chunks of equal length: W / target + (number of tiles) items at most, whatever the lengths are,
-// and no item longer than 2 S.  Items are numbered request by request, tile by tile.
+// The split.  Request i: R_i = G * T_i rows in rt_i tiles of TR, at most nb_i blocks of 64 keys a tile.  A tile is cut into C_i = ceil(nb_i / S) equal
+// chunks, S being the shortest of some lengths for which sum rt_i * C_i <= target, the workgroups that run at once: no workgroup works
+// longer than S, and none waits for a second round.  The lengths tried are multiples of W / target, W = sum rt_i * nb_i, at least min_blocks; where
+// none is long enough (more tiles than workgroups) the last, under which there are target + (number of tiles) items at most.  Items are
+// numbered request by request, tile by tile.
 // ---------------------------------------------------------------------------------------------
 struct Work { int req, seq, q0, T, L, first, tile, chunk, chunks; };
 
@@ -44,59 +45,113 @@ static __device__ __forceinline__ void request_tiles(const PagedAttnArgs& a, int
     if (a.window) keys = (int)min((long)keys, (long)a.window + TR / a.G + 65);
     *nb = (keys + 63) >> 6;
 }
+static __device__ __forceinline__ int chunks_of(const PagedAttnArgs& a, int nb, float S) {
+    return min(max((int)ceilf((float)nb / S - 1e-3f), 1), a.cmax);
+}
+#define TRIES 8
+// what item `item` is, in scalars; false: there are fewer.  Up to 64 requests every wave looks at all of them by itself.
 template <int NTH, int TR>
 static __device__ __forceinline__ bool schedule(const PagedAttnArgs& a, int item, Work* out) {
     __shared__ float fsum[NTH / 64];
-    __shared__ int isum[NTH / 64];
+    __shared__ int isum[TRIES][NTH / 64];
     __shared__ Work found;
     __shared__ int have;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    if (tid == 0) have = 0;
-    int seq, q0, T, L, rt = 0, nb = 0;
-    float w = 0.f;
-    for (int i0 = 0; i0 < a.n; i0 += NTH) {
-        if (i0 + tid < a.n) {
-            request_shape(a, i0 + tid, &seq, &q0, &T, &L);
-            request_tiles<TR>(a, T, L, &rt, &nb);
-            w += (float)rt * (float)nb;
+    const float tries[TRIES] = {1.f, 1.06f, 1.13f, 1.22f, 1.35f, 1.55f, 1.85f, 2.5f};
+    const bool few = a.n <= 64;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, me = few ? lane : tid, step = few ? 64 : NTH;
+    int seq = 0, q0 = 0, T = 0, L = 0, rt = 0, nb = 0;
+    float W = 0.f;
+    for (int i = me; i < a.n; i += step) {
+        request_shape(a, i, &seq, &q0, &T, &L);
+        request_tiles<TR>(a, T, L, &rt, &nb);
+        W += (float)rt * (float)nb;
+    }
+    W = wave_sum(W);
+    if (!few) {
+        if (tid == 0) have = 0;
+        if (lane == 0) fsum[wave] = W;
+        __syncthreads();
+        W = 0.f;
+#pragma unroll
+        for (int k = 0; k < NTH / 64; ++k) W += fsum[k];
+    }
+    const float S0 = W / (float)a.target;
+    int cnt[TRIES];
+#pragma unroll
+    for (int k = 0; k < TRIES; ++k) cnt[k] = 0;
+    for (int i = me; i < a.n; i += step) {
+        if (a.n > step) { request_shape(a, i, &seq, &q0, &T, &L); request_tiles<TR>(a, T, L, &rt, &nb); }
+#pragma unroll
+        for (int k = 0; k < TRIES; ++k) cnt[k] += rt * chunks_of(a, nb, fmaxf((float)a.min_blocks, S0 * tries[k]));
+    }
+#pragma unroll
+    for (int k = 0; k < TRIES; ++k)
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) cnt[k] += __shfl_xor(cnt[k], o, 64);
+    if (!few) {
+        if (lane == 0)
+#pragma unroll
+            for (int k = 0; k < TRIES; ++k) isum[k][wave] = cnt[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < TRIES; ++k) {
+            cnt[k] = 0;
+#pragma unroll
+            for (int x = 0; x < NTH / 64; ++x) cnt[k] += isum[k][x];
         }
     }
-    w = wave_sum(w);
-    if (lane == 0) fsum[wave] = w;
-    __syncthreads();
-    float all = 0.f;
+    float S = S0 * tries[TRIES - 1];
 #pragma unroll
-    for (int k = 0; k < NTH / 64; ++k) all += fsum[k];
-    const int S = max(a.min_blocks, (int)ceilf(fminf(all / (float)a.target, 1e9f)));
+    for (int k = TRIES - 2; k >= 0; --k)
+        if (cnt[k] <= a.target) S = S0 * tries[k];
+    S = fmaxf(S, (float)a.min_blocks);
     int base = 0;
-    for (int i0 = 0; i0 < a.n; i0 += NTH) {
-        int C = 1, items = 0;
-        if (a.n > NTH) {                                    // one request a thread: its numbers are still at hand
-            rt = nb = 0;
-            if (i0 + tid < a.n) { request_shape(a, i0 + tid, &seq, &q0, &T, &L); request_tiles<TR>(a, T, L, &rt, &nb); }
-        }
-        if (i0 + tid < a.n) { C = min(max(nb / S, 1), a.cmax); items = rt * C; }
+    Work f;
+    if (few) {
+        const int C = chunks_of(a, nb, S), items = me < a.n ? rt * C : 0;
         int x = items;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) { const int y = __shfl_up(x, o, 64); if (lane >= o) x += y; }
-        if (lane == 63) isum[wave] = x;
-        __syncthreads();
-        int before = base;
-        for (int k = 0; k < NTH / 64; ++k) { if (k < wave) before += isum[k]; base += isum[k]; }
-        const int k = item - (before + x - items);
-        if (k >= 0 && k < items) {
-            found = {i0 + tid, seq, q0, T, L, item - k, k / C, k % C, C};
-            have = 1;
+        const int k = item - (x - items);
+        const unsigned long long at = __ballot(k >= 0 && k < items);
+        if (!at) return false;
+        const int src = __ffsll(at) - 1;
+        f = {src, seq, q0, T, L, item - k, k / C, k % C, C};
+        out->req = src; out->seq = __builtin_amdgcn_readlane(f.seq, src); out->q0 = __builtin_amdgcn_readlane(f.q0, src);
+        out->T = __builtin_amdgcn_readlane(f.T, src); out->L = __builtin_amdgcn_readlane(f.L, src); out->first = __builtin_amdgcn_readlane(f.first, src);
+        out->tile = __builtin_amdgcn_readlane(f.tile, src); out->chunk = __builtin_amdgcn_readlane(f.chunk, src);
+        out->chunks = __builtin_amdgcn_readlane(f.chunks, src);
+    } else {
+        for (int i0 = 0; i0 < a.n; i0 += NTH) {
+            int C = 1, items = 0;
+            if (a.n > NTH) {                                // one request a thread: its numbers are still at hand
+                rt = nb = 0;
+                if (i0 + tid < a.n) { request_shape(a, i0 + tid, &seq, &q0, &T, &L); request_tiles<TR>(a, T, L, &rt, &nb); }
+            }
+            if (i0 + tid < a.n) { C = chunks_of(a, nb, S); items = rt * C; }
+            int x = items;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) { const int y = __shfl_up(x, o, 64); if (lane >= o) x += y; }
+            __syncthreads();
+            if (lane == 63) isum[0][wave] = x;
+            __syncthreads();
+            int before = base;
+            for (int k = 0; k < NTH / 64; ++k) { if (k < wave) before += isum[0][k]; base += isum[0][k]; }
+            const int k = item - (before + x - items);
+            if (k >= 0 && k < items) {
+                found = {i0 + tid, seq, q0, T, L, item - k, k / C, k % C, C};
+                have = 1;
+            }
+            __syncthreads();
+            if (have) break;
         }
-        __syncthreads();
-        if (have) break;
+        if (!have) return false;
+        f = found;
+        out->req = __builtin_amdgcn_readfirstlane(f.req); out->seq = __builtin_amdgcn_readfirstlane(f.seq);
+        out->q0 = __builtin_amdgcn_readfirstlane(f.q0); out->T = __builtin_amdgcn_readfirstlane(f.T); out->L = __builtin_amdgcn_readfirstlane(f.L);
+        out->first = __builtin_amdgcn_readfirstlane(f.first); out->tile = __builtin_amdgcn_readfirstlane(f.tile);
+        out->chunk = __builtin_amdgcn_readfirstlane(f.chunk); out->chunks = __builtin_amdgcn_readfirstlane(f.chunks);
     }
-    if (!have) return false;
-    const Work f = found;                                   // the same in all: scalars
-    out->req = __builtin_amdgcn_readfirstlane(f.req); out->seq = __builtin_amdgcn_readfirstlane(f.seq);
-    out->q0 = __builtin_amdgcn_readfirstlane(f.q0); out->T = __builtin_amdgcn_readfirstlane(f.T); out->L = __builtin_amdgcn_readfirstlane(f.L);
-    out->first = __builtin_amdgcn_readfirstlane(f.first); out->tile = __builtin_amdgcn_readfirstlane(f.tile);
-    out->chunk = __builtin_amdgcn_readfirstlane(f.chunk); out->chunks = __builtin_amdgcn_readfirstlane(f.chunks);
     // for the join: where a request's partial results are
     if (item == out->first && (int)blockIdx.x == item * a.kv_heads && tid == 0 && a.cmax > 1) { a.info[2 * out->req] = out->first; a.info[2 * out->req + 1] = out->chunks; }
     return true;
@@ -410,7 +465,7 @@ __global__ __launch_bounds__(256) void paged_attn_rows_kernel(PagedAttnArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// Many rows (frames, prompts): bound by the matrix cores and the exponentials.  A workgroup's four waves have 32 rows each and share blocks of
+// Many rows (frames, prompts): bound by the matrix cores and the exponentials.  A workgroup's four waves have 16 NT rows each and share blocks of
 // 64 keys, K and V double-buffered in LDS: the next block is under way while this one is computed, with one barrier a block.  bf16 pages go
 // straight to LDS (buffer_load ... lds, 1 KiB of contiguous rows an instruction), e4m3 through registers, where they become bf16.  In LDS a row's
 // 16-byte chunks are permuted by its number: sixteen rows read at one column, or eight rows at two, touch every bank once.
@@ -430,9 +485,9 @@ static __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t from, 
 #endif
 }
 
-template <int D, bool E4M3>
+template <int D, bool E4M3, int NT>
 __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a) {
-    constexpr int KSQ = D / 32, DT = D / 16, TR = 128, BLK = 64 * D;
+    constexpr int KSQ = D / 32, DT = D / 16, TR = 64 * NT, BLK = 64 * D;
     using LD = TileLds<D>;
     extern __shared__ __attribute__((aligned(16))) bf16 kv[];             // [buffer][K, V][64][D]
     __shared__ int odd_s[2];
@@ -447,13 +502,13 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
     const int b0 = w.chunk * sp.S, b1 = min(sp.nb, b0 + sp.S);
     if (b0 >= b1 && w.chunks > 1) { no_keys<TR>(a, item, hk); return; }
     const int R = w.T * a.G, base_pos = w.L - w.T;
-    const int row0 = w.tile * TR + wave * 32;
+    const int row0 = w.tile * TR + wave * 16 * NT;
     const bool wave_on = row0 < R;
 
-    int pos[2];
-    bf16x8 qf[2][KSQ];
+    int pos[NT];
+    bf16x8 qf[NT][KSQ];
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
+    for (int nt = 0; nt < NT; ++nt) {
         const int r = min(row0 + nt * 16 + r16, R - 1), t = r / a.G, g = r - t * a.G;
         pos[nt] = base_pos + t;
         const bf16* qp = a.q + (long)(w.q0 + t) * a.ldq + (long)(hk * a.G + g) * a.hd;
@@ -467,13 +522,13 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
     }
     // the positions of the workgroup's rows, and of the wave's
     const int pos_lo = base_pos + w.tile * TR / a.G, pos_hi = base_pos + min((w.tile * TR + TR - 1) / a.G, w.T - 1);
-    const int wpos_lo = base_pos + min(row0, R - 1) / a.G, wpos_hi = base_pos + min(row0 + 31, R - 1) / a.G;
+    const int wpos_lo = base_pos + min(row0, R - 1) / a.G, wpos_hi = base_pos + min(row0 + 16 * NT - 1, R - 1) / a.G;
     const float c2 = a.scale * (E4M3 && a.k_scale ? a.k_scale[hk] : 1.f) * 1.4426950408889634f;
 
-    f32x4 o[2][DT], lacc[2];
-    float m_run[2];
+    f32x4 o[NT][DT], lacc[NT];
+    float m_run[NT];
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
+    for (int nt = 0; nt < NT; ++nt) {
         m_run[nt] = -INFINITY; lacc[nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < DT; ++i) o[nt][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -540,9 +595,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
     // the wave's own page a block ahead; all four of the block itself, for the mask
     const bool one_page = a.lps >= 6;                       // a block lies in one page
     int mine = look_up(sp.first + b0 * 64, wave);
-    int p0, p1, p2, p3;
+    int p0, p1 = 0, p2 = 0, p3 = 0;
     auto look_up_all = [&](int key0) {
-        p0 = p1 = p2 = p3 = look_up(key0, 0);
+        p0 = look_up(key0, 0);
         if (!one_page) { p1 = look_up(key0, 1); p2 = look_up(key0, 2); p3 = look_up(key0, 3); }
     };
     look_up_all(sp.first + b0 * 64);
@@ -552,7 +607,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
         const int key0 = sp.first + b * 64;
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();                       // this block is in LDS, the other buffer is free
-        const unsigned bad = (no_page(p0) ? 1u : 0u) | (no_page(p1) ? 2u : 0u) | (no_page(p2) ? 4u : 0u) | (no_page(p3) ? 8u : 0u);
+        unsigned bad = 0;
+        if (no_page(p0) || no_page(p1) || no_page(p2) || no_page(p3))
+            bad = one_page ? 15 : (no_page(p0) ? 1u : 0u) | (no_page(p1) ? 2u : 0u) | (no_page(p2) ? 4u : 0u) | (no_page(p3) ? 8u : 0u);
         const bool plain = !bad && key0 + 63 <= pos_lo && (!a.window || key0 > pos_hi - a.window);             // every row sees every key
         bool odd = false;
         if (!plain) {
@@ -579,20 +636,27 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
         if (wave_on && key0 <= wpos_hi && (!a.window || key0 + 63 > wpos_lo - a.window)) {
             const bf16* ks_ = kv + buf * 2 * BLK;
             const bf16* vs_ = ks_ + BLK;
-            f32x4 s[2][4];
+            f32x4 s[NT][4];
 #pragma unroll
             for (int kt = 0; kt < 4; ++kt) {
-                s[0][kt] = s[1][kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) s[nt][kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int ks = 0; ks < KSQ; ++ks) {
                     const bf16x8 kf = *(const bf16x8*)&ks_[LD::k_slot(kt * 16 + r16, ks * 4 + q4)];
-                    s[0][kt] = mfma16(kf, qf[0][ks], s[0][kt]);
-                    s[1][kt] = mfma16(kf, qf[1][ks], s[1][kt]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) s[nt][kt] = mfma16(kf, qf[nt][ks], s[nt][kt]);
                 }
+            }
+            __builtin_amdgcn_sched_group_barrier(0x100, 2 * KSQ, 0);      // K fragments a key tile ahead of their products
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt) {
+                __builtin_amdgcn_sched_group_barrier(0x8, NT * KSQ, 0);
+                if (kt < 2) __builtin_amdgcn_sched_group_barrier(0x100, KSQ, 0);
             }
             if (!plain && (bad || key0 + 63 > wpos_lo || (a.window && key0 <= wpos_hi - a.window))) {
 #pragma unroll
-                for (int nt = 0; nt < 2; ++nt) {
+                for (int nt = 0; nt < NT; ++nt) {
                     int ahead = pos[nt] - key0 - 4 * q4;    // the last key the row sees, from this lane's first
                     asm volatile("" : "+v"(ahead));         // (computed here, not kept in registers through the loop)
                     const int least = a.window ? ahead - a.window : -0x40000000;
@@ -605,9 +669,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
                         }
                 }
             }
-            bf16x8 pb[2][2];
+            bf16x8 pb[NT][2];
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt) {
+            for (int nt = 0; nt < NT; ++nt) {
                 // exponentials against the running reference; only where one of them exceeds 2^8, or a row has no reference yet, is the
                 // row's maximum looked for
                 float p[4][4], top = 0.f;
@@ -660,9 +724,17 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
 #pragma unroll
                     for (int kp_ = 0; kp_ < 2; ++kp_) {
                         const bf16x8 vf = v_frag(dt, kp_);
-                        o[0][dt] = mfma16(vf, pb[0][kp_], o[0][dt]);
-                        o[1][dt] = mfma16(vf, pb[1][kp_], o[1][dt]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) o[nt][dt] = mfma16(vf, pb[nt][kp_], o[nt][dt]);
                     }
+                if constexpr (!E4M3) {                      // (the registers of an e4m3 block under way leave no room)
+                    __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);    // V fragments two channel tiles ahead
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) {
+                        __builtin_amdgcn_sched_group_barrier(0x8, 2 * NT, 0);
+                        if (dt + 2 < DT) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+                    }
+                }
             } else {
                 for (int p = wpos_lo; p <= wpos_hi; ++p) {  // each position's rows on their own, with the keys they see (0 * inf is no zero)
                     int ahead = p - key0 - 4 * q4;
@@ -679,7 +751,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
                                 if (j > ahead || j <= least) vf[e] = 0;
                             }
 #pragma unroll
-                            for (int nt = 0; nt < 2; ++nt) {
+                            for (int nt = 0; nt < NT; ++nt) {
                                 const f32x4 x = mfma16(vf, pb[nt][kp_], o[nt][dt]);
                                 o[nt][dt] = pos[nt] == p ? x : o[nt][dt];
                             }
@@ -693,7 +765,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
 
     const float vsc = E4M3 && a.v_scale ? a.v_scale[hk] : 1.f;
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
+    for (int nt = 0; nt < NT; ++nt) {
         const int r = row0 + nt * 16 + r16;
         if (r >= R) continue;
         const float l = lacc[nt][0];
@@ -705,7 +777,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
             for (int dt = 0; dt < DT; ++dt)
                 if (dt * 16 < a.hd) *(bf16x4*)(op + dt * 16) = (bf16x4){f2bf(o[nt][dt][0] * inv), f2bf(o[nt][dt][1] * inv), f2bf(o[nt][dt][2] * inv), f2bf(o[nt][dt][3] * inv)};
         } else {
-            const long pr = ((long)item * a.kv_heads + hk) * TR + wave * 32 + nt * 16 + r16;
+            const long pr = ((long)item * a.kv_heads + hk) * TR + (wave * NT + nt) * 16 + r16;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) *(f32x4*)&a.part_o[pr * D + dt * 16 + 4 * q4] = o[nt][dt];
             if (q4 == 0) { a.part_ml[pr * 2] = m_run[nt]; a.part_ml[pr * 2 + 1] = l; }
@@ -714,20 +786,22 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
 }
 
 // ---------------------------------------------------------------------------------------------
-// Joins the chunks of split rows, a wave for each token and query head (or, of many tokens, for each token: most then have nothing to join).
-// A lane knows one chunk's maximum and sum, so the weights of 64 chunks take one load; then 64 / (D / 4) partial rows are added at a time.  What
-// bounds it is the chain request -> item -> maximum -> output: the request is found by counting, not by bisection.
+// Joins the chunks of split rows: a wave for each token (of many tokens most have nothing to join), for each token and query head, or, where that
+// leaves the chip empty, four waves for each token and head, which share its chunks.  A lane knows one chunk's maximum and sum, so the weights of
+// 64 chunks take one load; then 64 / (D / 4) partial rows are added at a time.  What bounds it is the chain request -> item -> maximum -> output:
+// the request is found by counting, not by bisection.
 // ---------------------------------------------------------------------------------------------
-template <int D, int TR>
+template <int D, int TR, int WAVES>
 __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a, int e4m3, int heads_each) {
-    constexpr int LPR = D / 4, AT = 64 / LPR;               // lanes of a row, rows at a time
-    const int heads = a.kv_heads * a.G, groups = heads / heads_each;
-    const int unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
+    constexpr int LPR = D / 4, AT = 64 / LPR, FLY = WAVES == 4 ? 8 : 4;   // lanes of a row, rows at a time, loads under way
+    __shared__ float sh_m[4], sh_l[4];
+    __shared__ f32x4 sh_o[4][LPR];
+    const int heads = a.kv_heads * a.G, groups = heads / heads_each, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int unit = WAVES == 4 ? blockIdx.x : blockIdx.x * 4 + wave, lane = threadIdx.x & 63;
     const int tok = unit / groups;
     if (tok >= a.n_tokens) return;
     int req = 0;
     if (a.n <= 512) {
-#pragma unroll 4
         for (int i0 = 0; i0 < a.n; i0 += 64) req += __popcll(__ballot(i0 + lane < a.n && a.cu[min(i0 + lane, a.n - 1) + 1] <= tok));
     } else {
         int hi = a.n;
@@ -737,37 +811,64 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a, i
     const int q0 = a.cu[req], T = a.cu[req + 1] - q0, seq = a.seqs[req], first = a.info[2 * req], chunks = a.info[2 * req + 1];
     if (tok < q0 || (unsigned)seq >= (unsigned)a.max_seqs || chunks <= 1) return;
     const int rt = (int)(((long)T * a.G + TR - 1) / TR), col = lane % LPR * 4, sub = lane / LPR;
+    const int each = (chunks + WAVES - 1) / WAVES, c_lo = WAVES == 4 ? wave * each : 0, c_hi = min(chunks, c_lo + each);
     for (int h = unit % groups * heads_each, end = h + heads_each; h < end; ++h) {
         const int hk = h / a.G, r = (tok - q0) * a.G + h - hk * a.G, tile = r / TR;
-        const long item = first + (long)(TR == 128 ? rt - 1 - tile : tile) * chunks;
+        const long item = first + (long)(TR > 16 ? rt - 1 - tile : tile) * chunks;         // (the tile kernel takes a request's tiles from the last)
         if (item < 0 || item + chunks > a.grid_items) return;             // (a cu that is no running sum)
         const long step = (long)a.kv_heads * TR, p0 = (item * a.kv_heads + hk) * TR + (r - tile * TR);
         float M = -INFINITY, l = 0.f;
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-        for (int c0 = 0; c0 < chunks; c0 += 64) {
+        for (int c0 = c_lo; c0 < c_hi; c0 += 64) {
             float m = -INFINITY, ls = 0.f;
-            if (c0 + lane < chunks) { const float2 x = *(const float2*)&a.part_ml[(p0 + (c0 + lane) * step) * 2]; m = x.x; ls = x.y; }
+            if (c0 + lane < c_hi) { const float2 x = *(const float2*)&a.part_ml[(p0 + (c0 + lane) * step) * 2]; m = x.x; ls = x.y; }
             const float Mn = fmaxf(M, wave_max(m)), ref = Mn == -INFINITY ? 0.f : Mn;
             const float f = __builtin_amdgcn_exp2f(m - ref), old = __builtin_amdgcn_exp2f(M - ref);
             l = l * old + wave_sum(ls * f);
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[e] *= old;
             M = Mn;
-            const int cn = min(64, chunks - c0);
-#pragma unroll 4
-            for (int c = 0; c < cn; c += AT) {
-                const float fc = __shfl(f, min(c + sub, 63), 64), mc = __shfl(m, min(c + sub, 63), 64);
-                if (c + sub < cn && mc != -INFINITY) {
-                    const f32x4 v = *(const f32x4*)&a.part_o[(p0 + (c0 + c + sub) * step) * D + col];
+            const int cn = min(64, c_hi - c0);
+            for (int c = 0; c < cn; c += FLY * AT) {
+                f32x4 v[FLY];
+                float fc[FLY];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[e] += v[e] * fc;
+                for (int i = 0; i < FLY; ++i) {
+                    const int x = min(c + i * AT + sub, 63);
+                    const float mx = __shfl(m, x, 64), fx = __shfl(f, x, 64);           // (all lanes: a lane that is off gives nothing)
+                    const bool some = c + i * AT + sub < cn && mx != -INFINITY;
+                    fc[i] = some ? fx : 0.f;
+                    v[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+                    if (some) v[i] = *(const f32x4*)&a.part_o[(p0 + (c0 + x) * step) * D + col];
                 }
+#pragma unroll
+                for (int i = 0; i < FLY; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[e] += v[i][e] * fc[i];
             }
         }
 #pragma unroll
         for (int o = LPR; o < 64; o <<= 1)
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], o, 64);
+        if constexpr (WAVES == 4) {                          // (one head a workgroup: every wave is here)
+            if (lane == 0) { sh_m[wave] = M; sh_l[wave] = l; }
+            if (sub == 0) sh_o[wave][lane] = acc;
+            __syncthreads();
+            if (wave) return;
+            M = fmaxf(fmaxf(sh_m[0], sh_m[1]), fmaxf(sh_m[2], sh_m[3]));
+            const float ref = M == -INFINITY ? 0.f : M;
+            l = 0.f;
+            acc = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const float f = __builtin_amdgcn_exp2f(sh_m[x] - ref);
+                l += sh_l[x] * f;
+                const f32x4 v = sh_o[x][lane % LPR];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[e] += v[e] * f;
+            }
+        }
         const float inv = l > 0.f ? (e4m3 && a.v_scale ? a.v_scale[hk] : 1.f) / l : l == 0.f ? 0.f : l;
         if (sub == 0 && col < a.hd)
             *(bf16x4*)(a.out + (long)tok * a.ldo + (long)h * a.hd + col) = (bf16x4){f2bf(acc[0] * inv), f2bf(acc[1] * inv), f2bf(acc[2] * inv), f2bf(acc[3] * inv)};
@@ -775,11 +876,10 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a, i
 }
 
 // ---------------------------------------------------------------------------------------------
-// ---------------------------------------------------------------------------------------------
-// Sixteen rows a tile for a token (G rows of a key-value head), 32 for some drafted ones, 128 beyond: the matrix cores are then what counts.
+// Sixteen rows a tile for a token (the G rows of a key-value head), 64 for drafted ones, 128 beyond.
 static int rows_of_tile(const PagedAttnArgs* a, int max_q) {
     const long rows = (long)(max_q > 0 ? max_q : (a->n_tokens + a->n - 1) / (a->n > 0 ? a->n : 1)) * a->G;
-    return rows <= 16 ? 16 : rows <= 32 ? 32 : 128;
+    return rows <= 16 ? 16 : rows <= 64 ? 64 : 128;
 }
 static int template_dim(const PagedAttnArgs* a) { return a->hd <= 64 ? 64 : 128; }
 
@@ -788,14 +888,14 @@ size_t paged_partial_floats(const PagedAttnArgs* a) { return (size_t)a->grid_ite
 size_t paged_attention_plan(PagedAttnArgs* a, int n_cus, int max_q, int max_len) {
     const int TR = a->tile_rows = rows_of_tile(a, max_q);
     const long tiles = (long)a->n_tokens * a->G / TR + a->n;              // of one key-value head, at most
-    const int per_cu = TR == 128 ? 2 : 4;                                  // workgroups that run on a CU at once
+    const int per_cu = TR > 16 ? 2 : 4;                                  // workgroups that run on a CU at once
     a->target = (per_cu * n_cus + a->kv_heads - 1) / a->kv_heads;
     a->min_blocks = 2;                                                    // 128 keys: one block of 32 for each of the four waves
     long cap = (long)a->max_blocks << a->lps;
     if (max_len > 0 && max_len < cap) cap = max_len;
     const long nb = (cap + 63) / 64;
     a->cmax = (int)(nb / a->min_blocks < 1 ? 1 : nb / a->min_blocks);
-    const long by_split = a->target + a->target / 1024 + 8 + tiles, by_len = tiles * a->cmax;
+    const long by_split = a->target + tiles, by_len = tiles * a->cmax;
     a->grid_items = (int)(by_len < by_split ? by_len : by_split);
     if (a->cmax == 1) return 0;
     return (paged_partial_floats(a) + (size_t)a->grid_items * a->kv_heads * TR * 2) * sizeof(float) + (size_t)a->n * 2 * sizeof(int);
@@ -804,19 +904,21 @@ size_t paged_attention_plan(PagedAttnArgs* a, int n_cus, int max_q, int max_len)
 template <int D, bool E4M3, int TR>
 static hipError_t launch(const PagedAttnArgs* a, hipStream_t st) {
     const int grid = a->grid_items * a->kv_heads;
-    if constexpr (TR == 128) paged_attn_tile_kernel<D, E4M3><<<grid, 256, 4 * 64 * D * sizeof(bf16), st>>>(*a);
+    if constexpr (TR > 16) paged_attn_tile_kernel<D, E4M3, TR / 64><<<grid, 256, 4 * 64 * D * sizeof(bf16), st>>>(*a);
     else paged_attn_rows_kernel<D, E4M3, TR / 16><<<grid, 256, 0, st>>>(*a);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && a->cmax > 1) {
         const int heads = a->kv_heads * a->G, each = a->n_tokens >= 2048 ? heads : 1;
-        paged_attn_join_kernel<D, TR><<<(int)(((long)a->n_tokens * (heads / each) + 3) / 4), 256, 0, st>>>(*a, E4M3, each);
+        const long rows = (long)a->n_tokens * (heads / each);
+        if (rows <= 1024) paged_attn_join_kernel<D, TR, 4><<<(int)rows, 256, 0, st>>>(*a, E4M3, each);
+        else paged_attn_join_kernel<D, TR, 1><<<(int)((rows + 3) / 4), 256, 0, st>>>(*a, E4M3, each);
         e = hipGetLastError();
     }
     return e;
 }
 template <int D, bool E4M3>
 static hipError_t launch(const PagedAttnArgs* a, hipStream_t st) {
-    return a->tile_rows == 16 ? launch<D, E4M3, 16>(a, st) : a->tile_rows == 32 ? launch<D, E4M3, 32>(a, st) : launch<D, E4M3, 128>(a, st);
+    return a->tile_rows == 16 ? launch<D, E4M3, 16>(a, st) : a->tile_rows == 64 ? launch<D, E4M3, 64>(a, st) : launch<D, E4M3, 128>(a, st);
 }
 hipError_t paged_attention(const PagedAttnArgs* a, int e4m3, hipStream_t st) {
     if (template_dim(a) == 64) return e4m3 ? launch<64, true>(a, st) : launch<64, false>(a, st);
