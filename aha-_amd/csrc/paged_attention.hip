@@ -48,6 +48,20 @@ static __device__ __forceinline__ void request_tiles(const PagedAttnArgs& a, int
 static __device__ __forceinline__ int chunks_of(const PagedAttnArgs& a, int nb, float S) {
     return min(max((int)ceilf((float)nb / S - 1e-3f), 1), a.cmax);
 }
+// running sum over the wave's lanes (data-parallel moves: no trip through LDS); the last lane has the total
+template <class T>
+static __device__ __forceinline__ T wave_scan(T x) {
+    static_assert(sizeof(T) == 4, "");
+#define PAGED_ADD(ctrl, rows) x += __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), ctrl, rows, 0xf, false))
+    PAGED_ADD(0x111, 0xf); PAGED_ADD(0x112, 0xf); PAGED_ADD(0x114, 0xf); PAGED_ADD(0x118, 0xf);       // within rows of sixteen
+    PAGED_ADD(0x142, 0xa); PAGED_ADD(0x143, 0xc);                                                    // the last lane of the rows before
+#undef PAGED_ADD
+    return x;
+}
+template <class T>
+static __device__ __forceinline__ T wave_total(T x) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_scan(x)), 63));
+}
 #define TRIES 8
 // what item `item` is, in scalars; false: there are fewer.  Up to 64 requests every wave looks at all of them by itself.
 template <int NTH, int TR>
@@ -66,7 +80,7 @@ static __device__ __forceinline__ bool schedule(const PagedAttnArgs& a, int item
         request_tiles<TR>(a, T, L, &rt, &nb);
         W += (float)rt * (float)nb;
     }
-    W = wave_sum(W);
+    W = wave_total(W);
     if (!few) {
         if (tid == 0) have = 0;
         if (lane == 0) fsum[wave] = W;
@@ -85,9 +99,7 @@ static __device__ __forceinline__ bool schedule(const PagedAttnArgs& a, int item
         for (int k = 0; k < TRIES; ++k) cnt[k] += rt * chunks_of(a, nb, fmaxf((float)a.min_blocks, S0 * tries[k]));
     }
 #pragma unroll
-    for (int k = 0; k < TRIES; ++k)
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) cnt[k] += __shfl_xor(cnt[k], o, 64);
+    for (int k = 0; k < TRIES; ++k) cnt[k] = wave_total(cnt[k]);
     if (!few) {
         if (lane == 0)
 #pragma unroll
@@ -109,9 +121,7 @@ static __device__ __forceinline__ bool schedule(const PagedAttnArgs& a, int item
     Work f;
     if (few) {
         const int C = chunks_of(a, nb, S), items = me < a.n ? rt * C : 0;
-        int x = items;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) { const int y = __shfl_up(x, o, 64); if (lane >= o) x += y; }
+        const int x = wave_scan(items);
         const int k = item - (x - items);
         const unsigned long long at = __ballot(k >= 0 && k < items);
         if (!at) return false;
@@ -129,9 +139,7 @@ static __device__ __forceinline__ bool schedule(const PagedAttnArgs& a, int item
                 if (i0 + tid < a.n) { request_shape(a, i0 + tid, &seq, &q0, &T, &L); request_tiles<TR>(a, T, L, &rt, &nb); }
             }
             if (i0 + tid < a.n) { C = chunks_of(a, nb, S); items = rt * C; }
-            int x = items;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) { const int y = __shfl_up(x, o, 64); if (lane >= o) x += y; }
+            const int x = wave_scan(items);
             __syncthreads();
             if (lane == 63) isum[0][wave] = x;
             __syncthreads();
@@ -888,7 +896,7 @@ size_t paged_partial_floats(const PagedAttnArgs* a) { return (size_t)a->grid_ite
 size_t paged_attention_plan(PagedAttnArgs* a, int n_cus, int max_q, int max_len) {
     const int TR = a->tile_rows = rows_of_tile(a, max_q);
     const long tiles = (long)a->n_tokens * a->G / TR + a->n;              // of one key-value head, at most
-    const int per_cu = TR > 16 ? 2 : 4;                                  // workgroups that run on a CU at once
+    const int per_cu = 2;                                  // workgroups that run on a CU at once
     a->target = (per_cu * n_cus + a->kv_heads - 1) / a->kv_heads;
     a->min_blocks = 2;                                                    // 128 keys: one block of 32 for each of the four waves
     long cap = (long)a->max_blocks << a->lps;

@@ -191,8 +191,8 @@ static int threads_for(int work) { return work <= 256 ? 256 : work <= 512 ? 512 
 
 hipError_t paged_reserve(const PagedReserveArgs* a, hipStream_t st) {
     const int map = a->n_tokens <= 4 * PT_THREADS;             // four tokens a thread: beyond that a second launch over the chip
-    const int work = a->n > a->n_tokens || !map ? a->n : a->n_tokens;
-    paged_tables_kernel<true><<<1, threads_for(work), 0, st>>>(*a, map);
+    const int pages = (a->n_tokens >> a->t.lps) + a->n;        // at most: the longest of the loops
+    paged_tables_kernel<true><<<1, threads_for(map && a->n_tokens > pages ? a->n_tokens : pages), 0, st>>>(*a, map);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && !map) {
         paged_slots_kernel<<<(a->n_tokens + 255) / 256, 256, 0, st>>>(*a);
@@ -201,6 +201,6 @@ hipError_t paged_reserve(const PagedReserveArgs* a, hipStream_t st) {
     return e;
 }
 hipError_t paged_truncate(const PagedReserveArgs* a, hipStream_t st) {
-    paged_tables_kernel<false><<<1, threads_for(a->n), 0, st>>>(*a, 0);
+    paged_tables_kernel<false><<<1, threads_for(8 * a->n), 0, st>>>(*a, 0);          // (how many pages come back is not known here: eight a request)
     return hipGetLastError();
 }
