@@ -645,6 +645,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
             const bf16* ks_ = kv + buf * 2 * BLK;
             const bf16* vs_ = ks_ + BLK;
             f32x4 s[NT][4];
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int kt = 0; kt < 4; ++kt) {
 #pragma unroll
@@ -662,6 +663,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
                 __builtin_amdgcn_sched_group_barrier(0x8, NT * KSQ, 0);
                 if (kt < 2) __builtin_amdgcn_sched_group_barrier(0x100, KSQ, 0);
             }
+            __builtin_amdgcn_s_setprio(0);
             if (!plain && (bad || key0 + 63 > wpos_lo || (a.window && key0 <= wpos_hi - a.window))) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
@@ -726,6 +728,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
                 const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(vs_ + LD::v_slot(kp_ * 32 + 16 + vrow, dt * 2 + vch) + vin));
                 return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
             };
+            __builtin_amdgcn_s_setprio(1);
             if (!odd) {
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt)
@@ -767,6 +770,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
                 }
             }
         }
+        __builtin_amdgcn_s_setprio(0);
         if (b + 1 < b1) unstage(buf ^ 1);
     }
     if (!wave_on) return;
