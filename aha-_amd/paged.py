@@ -104,6 +104,8 @@ class PagedKVCache:
         h = shape[1] if len(shape) == 3 else shape[1] // D
         if heads is not None and h != heads:
             raise ValueError(f"{name}: {heads} heads are needed, not {h}")
+        if x.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} requires a gradient and nothing here has one: detach it, or call under torch.no_grad()")
         many = shape[0] > 1
         if stride[-1] != 1 or (len(shape) == 3 and h > 1 and stride[1] != D) or (many and stride[0] < h * D):
             if out:
@@ -112,6 +114,8 @@ class PagedKVCache:
         return x, h, stride[0] if many else h * D
 
     def _stream(self) -> int:
+        if self.device.type != "cuda":
+            raise AhaError("aha_amd needs a GPU: the product path has no CPU fallback")
         return torch._C._cuda_getCurrentRawStream(self.device.index)
 
     def _chk(self, rc: int):
@@ -189,7 +193,7 @@ class PagedKVCache:
         """Causal attention of the sequences' last tokens (rows cu[i] .. cu[i+1] of q are those of seqs[i]) over their pages -> bf16 [N, heads,
         head_dim].  `window`: the nearest keys only; `scale`: head_dim ** -0.5 by default; `max_q` / `max_len`: the most new tokens and keys of
         a request where the caller knows them (they choose kernel and split, never the result's meaning).  Rows of no request are left alone:
-        pass `out` where they matter."""
+        pass `out` where they matter (it may be q itself)."""
         q, heads, ldq = self._rows("q", q)
         n, N = seqs.shape[0], q.shape[0]
         sp, cp = self._ints("seqs", seqs), self._ints("cu", cu, n + 1)

@@ -378,7 +378,7 @@ int aha_paged_append(aha_paged* p, int layer, const void* q, int64_t ldq, int he
 /* out[t] = softmax(scale * q[t] K^T) V, bf16 [n_tokens][heads][head_dim]: rows cu_tokens[i] .. cu_tokens[i+1]-1 are the LAST tokens of sequence
  * seqs[i] (its keys are already appended) and see the keys at and before their position, the nearest `window` of them (0: all).  heads / kv_heads
  * query heads share a key-value head.  A row that sees no key is 0; rows of padding (negative sequence) and behind cu_tokens[n] are left as
- * they were.  A table entry that is no page hides its keys.  max_q, max_len: the most new tokens and keys of a request (0: not known); they choose the kernel
+ * they were.  A table entry that is no page hides its keys.  out may be q.  max_q, max_len: the most new tokens and keys of a request (0: not known); they choose the kernel
  * and the split of long sequences, results are right for any value.  workspace: aha_paged_attention_workspace bytes for the same sizes,
  * aligned to 16, used by this call only until its work is done (calls that may run at once need one each). */
 int aha_paged_attention_workspace(aha_paged* p, int heads, int n_tokens, int n, int max_q, int max_len, size_t* bytes);

@@ -423,6 +423,45 @@ def test_attention_scale_strides_and_sharp_rows():
     assert not bool(buf[:, :128].any()) and not bool(buf[:, 15 * 128:].any())
 
 
+@pytest.mark.parametrize("hints", [dict(max_q=1, max_len=1), dict(max_q=1), dict(max_len=16), dict(max_q=2, max_len=100), dict(max_q=10 ** 6, max_len=10 ** 9)])
+def test_wrong_hints_cost_time_not_results(hints):
+    lens, counts = [700, 90, 1500], [131, 1, 9]
+    c = filled(lens, 16, 28, 4, 128, "bf16", 17)
+    cu = ints([0, 131, 132, 141])
+    check_attention(c, randn(gen(18), 141, 28, 128).bfloat16(), ints(range(3)), cu, **hints)
+
+
+@pytest.mark.parametrize("T", [1, 6, 60])
+def test_attention_in_place_and_twice_over_one_sequence(T):
+    """out is q; the same sequence listed twice (each time its last tokens are meant)."""
+    c = filled([900, 33], 32, 14, 2, 64, "bf16", 19)
+    q = randn(gen(20), 2 * T + 1, 14, 64).bfloat16()
+    seqs, cu = ints([0, 1, 0]), ints([0, T, T + 1, 2 * T + 1])
+    want = check_attention(c, q, seqs, cu, max_q=T)
+    got = q.clone()
+    assert c.attention(0, got, seqs, cu, max_q=T, out=got) is got
+    assert torch.equal(got, want)
+
+
+def test_a_workspace_that_is_too_small_is_refused():
+    import ctypes as C
+    c = filled([4000], 16, 28, 4, 128, "bf16", 23)
+    q = randn(gen(24), 1, 28, 128).bfloat16()
+    need = C.c_size_t()
+    c._chk(c.lib.aha_paged_attention_workspace(c.handle, 28, 1, 1, 1, 4000, C.byref(need)))
+    assert need.value > 0
+    ws = torch.empty(need.value, dtype=torch.uint8, device=DEV)
+
+    def call(p, size):
+        s, cu, out = ints([0]), ints([0, 1]), torch.empty_like(q)
+        rc = c.lib.aha_paged_attention(c.handle, 0, q.data_ptr(), 28 * 128, 28, s.data_ptr(), cu.data_ptr(), 1, 1, 1, 4000, 0, 0.1, out.data_ptr(), 28 * 128, p, size, c._stream())
+        torch.cuda.synchronize()
+        return rc
+
+    assert call(ws.data_ptr(), need.value - 1) == -34 and call(None, need.value) == -34 and call(ws.data_ptr() + 4, need.value) == -22
+    assert call(ws.data_ptr(), need.value) == 0
+
+
 def test_many_requests():
     """More requests than a workgroup has threads: the split is worked out over several rounds."""
     rng = random.Random(3)

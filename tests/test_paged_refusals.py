@@ -129,3 +129,15 @@ def test_attention_refuses(monkeypatch):
     assert attend(heads=0) == -34 and attend(heads=6, ldq=192, ldo=192, N=1 << 24) == -34
     assert c.lib.aha_paged_attention_workspace(c.handle, 4, 3, -1, 1, 1, C.byref(b)) == -22
     assert c.lib.aha_paged_attention_workspace(c.handle, 4, 3, 2, 1, 1, None) == -22
+
+
+def test_no_cpu_fallback_and_no_gradient():
+    c = make()
+    seqs, counts = torch.zeros(2, dtype=I), torch.ones(2, dtype=I)
+    with pytest.raises(AhaError, match="GPU"):
+        c.reserve(seqs, counts, 4)
+    q = torch.zeros((3, 4, 32), dtype=torch.bfloat16, requires_grad=True)
+    with pytest.raises(ValueError, match="gradient"):
+        c.attention(0, q, seqs, torch.zeros(3, dtype=I))
+    with torch.no_grad(), pytest.raises(AhaError, match="GPU"):
+        c.append(0, q, q[:, :2], q[:, :2], torch.zeros(3, dtype=I))
