@@ -202,13 +202,13 @@ static __device__ __forceinline__ bf16x8 e4m3x8(unsigned lo, unsigned hi) {     
 }
 
 // ---------------------------------------------------------------------------------------------
-// Few rows (a token, some drafted ones): bound by the bytes of K and V.  A workgroup's four waves take blocks of 32 keys in turn, each with a
-// softmax of its own and no barrier in the loop, and are merged at the end.  NT tiles of 16 rows share every K and V fragment.  The matrix
-// cores have time to spare, so P goes into the product as two bf16 halves (high and remainder): no precision is lost to its rounding.
+// Few rows (one token: the G rows of a key-value head): bound by the bytes of K and V.  A workgroup's four waves take blocks of 32 keys in turn,
+// each with a softmax of its own and no barrier in the loop, and are merged at the end.  The matrix cores have time to spare, so P goes into
+// the product as two bf16 halves (high and remainder): no precision is lost to its rounding (2^-17 of p).
 // ---------------------------------------------------------------------------------------------
-template <int D, bool E4M3, int NT>
+template <int D, bool E4M3>
 __global__ __launch_bounds__(256) void paged_attn_rows_kernel(PagedAttnArgs a) {
-    constexpr int KSQ = D / 32, DT = D / 16, VST = D + 16, TR = 16 * NT;
+    constexpr int KSQ = D / 32, DT = D / 16, VST = D + 16, TR = 16;
     constexpr int NK = E4M3 ? KSQ / 2 : KSQ;               // 16-byte loads of one K tile a lane
     constexpr int NV = E4M3 ? D / 32 : D / 16;             // 16-byte loads of 32 V rows a lane
     constexpr int VCH = E4M3 ? D / 16 : D / 8;             // 16-byte chunks of a V row
@@ -225,35 +225,28 @@ __global__ __launch_bounds__(256) void paged_attn_rows_kernel(PagedAttnArgs a) {
     if (b0 >= b1 && w.chunks > 1) { no_keys<TR>(a, item, hk); return; }
     const int R = w.T * a.G, base_pos = w.L - w.T;
 
-    // rows of this lane (one a tile) and their queries
-    int pos[NT];
-    bf16x8 qf[NT][KSQ];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const int r = min(w.tile * TR + nt * 16 + r16, R - 1), t = r / a.G, g = r - t * a.G;
-        pos[nt] = base_pos + t;
-        const bf16* qp = a.q + (long)(w.q0 + t) * a.ldq + (long)(hk * a.G + g) * a.hd;
+    // this lane's row and its query
+    bf16x8 qf[KSQ];
+    const int my_r = min(w.tile * TR + r16, R - 1), my_t = my_r / a.G, pos = base_pos + my_t;
+    {
+        const bf16* qp = a.q + (long)(w.q0 + my_t) * a.ldq + (long)(hk * a.G + my_r - my_t * a.G) * a.hd;
         const bf16x8 z8 = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
         for (int ks = 0; ks < KSQ; ++ks) {
             // E4M3: a lane's 16 bytes of a K row are 16 channels, the operands of two products; the queries follow that order
             const int ch = E4M3 ? (ks >> 1) * 64 + q4 * 16 + (ks & 1) * 8 : ks * 32 + q4 * 8;
             const bf16x8 v = *(const bf16x8*)(qp + min(ch, a.hd - 8));
-            qf[nt][ks] = ch < a.hd ? v : z8;
+            qf[ks] = ch < a.hd ? v : z8;
         }
     }
     const int pos_min = base_pos + w.tile * TR / a.G, pos_max = base_pos + min((w.tile * TR + TR - 1) / a.G, w.T - 1);
     const bool one_pos = pos_min == pos_max;
     const float c2 = a.scale * (E4M3 && a.k_scale ? a.k_scale[hk] : 1.f) * 1.4426950408889634f;
 
-    f32x4 o[NT][DT];
-    float m_run[NT], l_run[NT];
+    f32x4 o[DT];
+    float m_run = -INFINITY, l_run = 0.f;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        m_run[nt] = -INFINITY; l_run[nt] = 0.f;
-#pragma unroll
-        for (int i = 0; i < DT; ++i) o[nt][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    }
+    for (int i = 0; i < DT; ++i) o[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
     constexpr int ES = E4M3 ? 1 : 2;
     const long head_bytes = ((long)a.hd << a.lps) * ES;     // one head of one page
@@ -326,12 +319,11 @@ __global__ __launch_bounds__(256) void paged_attn_rows_kernel(PagedAttnArgs a) {
             off[0] = tile_off(kn, &page_ok[0]); off[1] = tile_off(kn + 16, &page_ok[1]);
             load_v();
         }
-        // ---- scores: s[nt][kt][e] is row r16's with key key0 + 16 kt + 4 q4 + e
-        f32x4 s[NT][2];
+        // ---- scores: s[kt][e] is row r16's with key key0 + 16 kt + 4 q4 + e
+        f32x4 s[2];
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) s[nt][kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            s[kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < NK; ++i) {
                 bf16x8 k0, k1;
@@ -341,134 +333,116 @@ __global__ __launch_bounds__(256) void paged_attn_rows_kernel(PagedAttnArgs a) {
                     const bf16x8 z8 = {0, 0, 0, 0, 0, 0, 0, 0};
                     if ((i * 4 + q4) * 16 >= a.hd * ES) { k0 = z8; if constexpr (E4M3) k1 = z8; }
                 }
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    if constexpr (E4M3) {
-                        s[nt][kt] = mfma16(k0, qf[nt][2 * i], s[nt][kt]);
-                        s[nt][kt] = mfma16(k1, qf[nt][2 * i + 1], s[nt][kt]);
-                    } else s[nt][kt] = mfma16(k0, qf[nt][i], s[nt][kt]);
-                }
+                if constexpr (E4M3) {
+                    s[kt] = mfma16(k0, qf[2 * i], s[kt]);
+                    s[kt] = mfma16(k1, qf[2 * i + 1], s[kt]);
+                } else s[kt] = mfma16(k0, qf[i], s[kt]);
             }
         }
         if (kn < k_end) load_k();
         const bool any_odd = !plain && !one_pos && __any(odd);
-        bf16x8 ph[NT], pl[NT];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            if (!plain) {
-#pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int j = key0 + kt * 16 + 4 * q4 + e;
-                        const bool see = j <= pos[nt] && j < k_end && (kt ? ok1 : ok0) && (!a.window || j > pos[nt] - a.window);
-                        s[nt][kt][e] = see ? s[nt][kt][e] : -INFINITY;
-                    }
-            }
-            float mx = fmaxf(fmaxf(fmaxf(s[nt][0][0], s[nt][0][1]), fmaxf(s[nt][0][2], s[nt][0][3])),
-                             fmaxf(fmaxf(s[nt][1][0], s[nt][1][1]), fmaxf(s[nt][1][2], s[nt][1][3])));
-            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            const float m_new = fmaxf(m_run[nt], mx * c2);
-            const float ref = m_new == -INFINITY ? 0.f : m_new;           // a row that has seen nothing yet: 2^(-inf) = 0 throughout
-            const float alpha = __builtin_amdgcn_exp2f(m_run[nt] - ref);
-            float psum = 0.f;
+        if (!plain) {
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nt][kt][e], c2, -ref));
-                    psum += p;
-                    const bf16 hi = f2bf(p);
-                    ph[nt][kt * 4 + e] = hi;
-                    pl[nt][kt * 4 + e] = f2bf(p - bf2f(hi));
+                    const int j = key0 + kt * 16 + 4 * q4 + e;
+                    const bool see = j <= pos && j < k_end && (kt ? ok1 : ok0) && (!a.window || j > pos - a.window);
+                    s[kt][e] = see ? s[kt][e] : -INFINITY;
                 }
-            m_run[nt] = m_new;
-            l_run[nt] = l_run[nt] * alpha + psum;
-#pragma unroll
-            for (int i = 0; i < DT; ++i) o[nt][i] *= alpha;
         }
+        float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float m_new = fmaxf(m_run, mx * c2);
+        const float ref = m_new == -INFINITY ? 0.f : m_new;                // a row that has seen nothing yet: 2^(-inf) = 0 throughout
+        const float alpha = __builtin_amdgcn_exp2f(m_run - ref);
+        float psum = 0.f;
+        bf16x8 ph, pl;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][e], c2, -ref));
+                psum += p;
+                const bf16 hi = f2bf(p);
+                ph[kt * 4 + e] = hi;
+                pl[kt * 4 + e] = f2bf(p - bf2f(hi));
+            }
+        m_run = m_new;
+        l_run = l_run * alpha + psum;
+#pragma unroll
+        for (int i = 0; i < DT; ++i) o[i] *= alpha;
         // ---- O^T += V^T P^T: slot (q4, e) is key 4 q4 + e of the first tile, of the second from e = 4
         const int vrow = 4 * q4 + (r16 >> 2), vcol = 4 * (r16 & 3);
+        auto v_frag = [&](int dt) {
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(&vs[vrow * VST + dt * 16 + vcol]));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(&vs[(16 + vrow) * VST + dt * 16 + vcol]));
+            return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        };
         if (!any_odd) {
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(&vs[vrow * VST + dt * 16 + vcol]));
-                const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(&vs[(16 + vrow) * VST + dt * 16 + vcol]));
-                const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    o[nt][dt] = mfma16(vf, ph[nt], o[nt][dt]);
-                    o[nt][dt] = mfma16(vf, pl[nt], o[nt][dt]);
-                }
+                const bf16x8 vf = v_frag(dt);
+                o[dt] = mfma16(vf, ph, o[dt]);
+                o[dt] = mfma16(vf, pl, o[dt]);
             }
         } else {
             // 0 * inf would carry a value into rows that do not see its key: each position's rows on their own, with the keys they see
             for (int p = pos_min; p <= pos_max; ++p) {
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
-                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(&vs[vrow * VST + dt * 16 + vcol]));
-                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(&vs[(16 + vrow) * VST + dt * 16 + vcol]));
-                    bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                    bf16x8 vf = v_frag(dt);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const int j = key0 + (e >> 2) * 16 + 4 * q4 + (e & 3);
                         if (j > p || (a.window && j <= p - a.window)) vf[e] = 0;
                     }
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        f32x4 t = mfma16(vf, ph[nt], o[nt][dt]);
-                        t = mfma16(vf, pl[nt], t);
-                        o[nt][dt] = pos[nt] == p ? t : o[nt][dt];
-                    }
+                    f32x4 t = mfma16(vf, ph, o[dt]);
+                    t = mfma16(vf, pl, t);
+                    o[dt] = pos == p ? t : o[dt];
                 }
             }
         }
         asm volatile("" ::: "memory");
     }
 
-    // ---- merge the four waves: O of the sixteen rows of a tile in LDS, one after the other
-    constexpr int OST = D + 4;
+    // ---- merge the four waves: O of the sixteen rows in LDS
+    constexpr int OST = D + 4, E = D / 16;
     static_assert(4 * 16 * OST * 4 <= (int)sizeof(Vs), "the merge uses V's LDS");
     float* ob = (float*)&Vs[0][0];
-    const float vsc = E4M3 && a.v_scale ? a.v_scale[hk] : 1.f;
+    l_run += __shfl_xor(l_run, 16, 64);
+    l_run += __shfl_xor(l_run, 32, 64);
+    __syncthreads();
+    if (q4 == 0) { sm[wave][r16] = m_run; sl[wave][r16] = l_run; }
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        float l = l_run[nt];
-        l += __shfl_xor(l, 16, 64);
-        l += __shfl_xor(l, 32, 64);
-        __syncthreads();
-        if (q4 == 0) { sm[wave][r16] = m_run[nt]; sl[wave][r16] = l; }
+    for (int dt = 0; dt < DT; ++dt) *(f32x4*)&ob[(wave * 16 + r16) * OST + dt * 16 + 4 * q4] = o[dt];
+    __syncthreads();
+    const int row = tid >> 4, c = (tid & 15) * E, r = w.tile * TR + row;
+    const float M = fmaxf(fmaxf(sm[0][row], sm[1][row]), fmaxf(sm[2][row], sm[3][row])), ref = M == -INFINITY ? 0.f : M;
+    float acc[E], lsum = 0.f;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) *(f32x4*)&ob[(wave * 16 + r16) * OST + dt * 16 + 4 * q4] = o[nt][dt];
-        __syncthreads();
-        const int row = tid >> 4, c = (tid & 15) * (D / 16), r = w.tile * TR + nt * 16 + row;
-        float M = fmaxf(fmaxf(sm[0][row], sm[1][row]), fmaxf(sm[2][row], sm[3][row]));
-        const float ref = M == -INFINITY ? 0.f : M;
-        float acc[D / 16], lsum = 0.f;
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
 #pragma unroll
-        for (int e = 0; e < D / 16; ++e) acc[e] = 0.f;
+    for (int x = 0; x < 4; ++x) {
+        const float f = __builtin_amdgcn_exp2f(sm[x][row] - ref);
+        lsum += sl[x][row] * f;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const float f = __builtin_amdgcn_exp2f(sm[x][row] - ref);
-            lsum += sl[x][row] * f;
+        for (int e = 0; e < E; ++e) acc[e] += ob[(x * 16 + row) * OST + c + e] * f;
+    }
+    if (r >= R) return;
+    if (w.chunks == 1) {
+        // a row that sees no key is zero; NaN stays
+        const float inv = lsum > 0.f ? (E4M3 && a.v_scale ? a.v_scale[hk] : 1.f) / lsum : lsum == 0.f ? 0.f : lsum;
+        const int t = r / a.G;
+        bf16* op = a.out + (long)(w.q0 + t) * a.ldo + (long)(hk * a.G + r - t * a.G) * a.hd;
 #pragma unroll
-            for (int e = 0; e < D / 16; ++e) acc[e] += ob[(x * 16 + row) * OST + c + e] * f;
-        }
-        if (r < R) {
-            if (w.chunks == 1) {
-                const float inv = lsum > 0.f ? vsc / lsum : lsum == 0.f ? 0.f : lsum;          // a row that sees no key is zero; NaN stays
-                const int t = r / a.G, g = r - t * a.G;
-                bf16* op = a.out + (long)(w.q0 + t) * a.ldo + (long)(hk * a.G + g) * a.hd;
+        for (int e = 0; e < E; ++e) if (c + e < a.hd) op[c + e] = f2bf(acc[e] * inv);
+    } else {
+        const long pr = ((long)item * a.kv_heads + hk) * TR + row;
 #pragma unroll
-                for (int e = 0; e < D / 16; ++e) if (c + e < a.hd) op[c + e] = f2bf(acc[e] * inv);
-            } else {
-                const long pr = ((long)item * a.kv_heads + hk) * TR + nt * 16 + row;
-#pragma unroll
-                for (int e = 0; e < D / 16; ++e) a.part_o[pr * D + c + e] = acc[e];
-                if ((tid & 15) == 0) { a.part_ml[pr * 2] = M; a.part_ml[pr * 2 + 1] = lsum; }
-            }
-        }
+        for (int e = 0; e < E; ++e) a.part_o[pr * D + c + e] = acc[e];
+        if (c == 0) { a.part_ml[pr * 2] = M; a.part_ml[pr * 2 + 1] = lsum; }
     }
 }
 
@@ -888,7 +862,9 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a, i
 }
 
 // ---------------------------------------------------------------------------------------------
-// Sixteen rows a tile for a token (the G rows of a key-value head), 64 for drafted ones, 128 beyond.
+// Sixteen rows a tile for a token (the G rows of a key-value head), 64 for drafted ones, 128 beyond.  Sixteen requests over 5,000 keys, 28 / 4
+// heads of 128, in tiles of 16 / 64 / 128 rows: 2 tokens (14 rows) 38 / 38 / 39 us, 5 (35) 66 / 40 / 41, 9 (63) 66 / 44 / 44, 10 (70) 112 / 47 / 45;
+// e4m3, 7 tokens (49): 64 / 128 rows 36.5 / 39.8 us.
 static int rows_of_tile(const PagedAttnArgs* a, int max_q) {
     const long rows = (long)(max_q > 0 ? max_q : (a->n_tokens + a->n - 1) / (a->n > 0 ? a->n : 1)) * a->G;
     return rows <= 16 ? 16 : rows <= 64 ? 64 : 128;
@@ -900,9 +876,10 @@ size_t paged_partial_floats(const PagedAttnArgs* a) { return (size_t)a->grid_ite
 size_t paged_attention_plan(PagedAttnArgs* a, int n_cus, int max_q, int max_len) {
     const int TR = a->tile_rows = rows_of_tile(a, max_q);
     const long tiles = (long)a->n_tokens * a->G / TR + a->n;              // of one key-value head, at most
-    const int per_cu = 2;                                  // workgroups that run on a CU at once
-    a->target = (per_cu * n_cus + a->kv_heads - 1) / a->kv_heads;
-    a->min_blocks = 2;                                                    // 128 keys: one block of 32 for each of the four waves
+    // Two workgroups a CU: what registers and LDS let run at once, and fewer, longer ones leave less to join (four, for tokens, against two:
+    // sixteen over 12,000 keys 80.7 / 77.9 us, one over 32,000 29.3 / 22.7 us).
+    a->target = (2 * n_cus + a->kv_heads - 1) / a->kv_heads;
+    a->min_blocks = 2;                                                    // 128 keys: a block of 32 for each of four waves (64 keys at least: within 2 % either way)
     long cap = (long)a->max_blocks << a->lps;
     if (max_len > 0 && max_len < cap) cap = max_len;
     const long nb = (cap + 63) / 64;
@@ -917,9 +894,11 @@ template <int D, bool E4M3, int TR>
 static hipError_t launch(const PagedAttnArgs* a, hipStream_t st) {
     const int grid = a->grid_items * a->kv_heads;
     if constexpr (TR > 16) paged_attn_tile_kernel<D, E4M3, TR / 64><<<grid, 256, 4 * 64 * D * sizeof(bf16), st>>>(*a);
-    else paged_attn_rows_kernel<D, E4M3, TR / 16><<<grid, 256, 0, st>>>(*a);
+    else paged_attn_rows_kernel<D, E4M3><<<grid, 256, 0, st>>>(*a);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && a->cmax > 1) {
+        // of many tokens a wave looks at all heads of one: mostly there is nothing to join (8,192 tokens: 5 us, with a wave a head 35 us); of few
+        // rows four waves share the chunks (one token over 32,000 keys: 29 us, with one wave 67 us)
         const int heads = a->kv_heads * a->G, each = a->n_tokens >= 2048 ? heads : 1;
         const long rows = (long)a->n_tokens * (heads / each);
         if (rows <= 1024) paged_attn_join_kernel<D, TR, 4><<<(int)rows, 256, 0, st>>>(*a, E4M3, each);
