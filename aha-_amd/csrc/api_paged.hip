@@ -44,6 +44,16 @@ struct OnDevice {
 
 static bool aligned16(const void* x) { return ((uintptr_t)x & 15) == 0; }
 
+// Do rows of `a` (n of them, wa elements each, lda apart) and of `b` share an element?  Rows of one buffer may lie between each other (the columns of a
+// fused projection) if they have the same stride; with another one, ranges that meet are taken to.
+static bool rows_meet(const void* a, int64_t lda, int64_t wa, const void* b, int64_t ldb, int64_t wb, int64_t n) {
+    const int64_t x = (intptr_t)a / 2, y = (intptr_t)b / 2;               // (bf16 elements; addresses are below 2^63)
+    if (x + (n - 1) * lda + wa <= y || y + (n - 1) * ldb + wb <= x) return false;
+    if (n == 1 || lda != ldb) return true;
+    const int64_t off = ((y - x) % lda + lda) % lda;
+    return off < wa || off + wb > lda;
+}
+
 extern "C" const char* aha_paged_last_error(void) { return g_paged_err; }
 
 extern "C" int aha_paged_create(const aha_paged_desc* d, int device, aha_paged** out) {
@@ -76,6 +86,7 @@ extern "C" int aha_paged_reserve(aha_paged* p, const int32_t* seqs, const int32_
     if (!p || !cu_tokens || !status) return refuse(E_INVAL, "null argument");
     if (n < 0 || n_tokens < 0 || (n && (!seqs || !counts)) || (n_tokens && (!slots || !positions))) return refuse(E_INVAL, "null array or negative size");
     if (n > 2 * PAGED_MAX_SEQS) return refuse(E_RANGE, "more than %d requests", 2 * PAGED_MAX_SEQS);
+    if (n_tokens > 0x7fffffff - 4096) return refuse(E_RANGE, "too many tokens in one call");
     PagedReserveArgs a = {tables_of(p), seqs, counts, n, slots, positions, n_tokens, cu_tokens, status};
     RUN("paged reserve", paged_reserve(&a, (hipStream_t)st));
     return 0;
@@ -106,7 +117,10 @@ extern "C" int aha_paged_append(aha_paged* p, int layer, const void* q, int64_t 
     if (ldk % 8 || ldv % 8 || (heads && (ldq % 8 || ldqo % 8))) return refuse(E_RANGE, "row strides must be multiples of 8 elements");
     if (!aligned16(k) || !aligned16(v) || !aligned16(cos) || !aligned16(sin) || (heads && (!aligned16(q) || !aligned16(q_out))))
         return refuse(E_INVAL, "tensors must be aligned to 16 bytes");
-    if (heads && q == q_out && ldq != ldqo) return refuse(E_INVAL, "in place: ldq and ldqo must be equal");
+    if (heads && (q == q_out ? n_tokens > 1 && ldq != ldqo : rows_meet(q, ldq, qw, q_out, ldqo, qw, n_tokens)))
+        return refuse(E_INVAL, "q_out overlaps q: it must be q itself, ldq and ldqo equal, or lie elsewhere");
+    if (heads && (rows_meet(k, ldk, kw, q_out, ldqo, qw, n_tokens) || rows_meet(v, ldv, kw, q_out, ldqo, qw, n_tokens)))
+        return refuse(E_INVAL, "q_out overlaps k or v");
     if ((int64_t)n_tokens * (heads + 2 * d.kv_heads) * (d.head_dim / 16) > 0x7fffffff) return refuse(E_RANGE, "too many tokens in one call");
     PagedAppendArgs a;
     a.q = (const bf16*)q; a.k = (const bf16*)k; a.v = (const bf16*)v; a.ldq = ldq; a.ldk = ldk; a.ldv = ldv;
@@ -130,12 +144,16 @@ static int cus_of(aha_paged* p, int* out) {
     *out = n;
     return 0;
 }
-static int attention_args(aha_paged* p, int heads, int n_tokens, int n, int max_q, int max_len, PagedAttnArgs* a, size_t* bytes) {
+static int attention_sizes(const aha_paged* p, int heads, int n_tokens, int n, int max_q, int max_len) {
     const aha_paged_desc& d = p->d;
     if (n_tokens < 0 || n < 0 || max_q < 0 || max_len < 0) return refuse(E_INVAL, "negative size");
     if (heads < 1 || heads > 4096 || heads % d.kv_heads) return refuse(E_RANGE, "heads must be a multiple of the cache's key-value heads, at most 4096");
     if (n > 2 * PAGED_MAX_SEQS) return refuse(E_RANGE, "more than %d requests", 2 * PAGED_MAX_SEQS);
     if ((int64_t)n_tokens * heads > 0xffffff || (int64_t)n * d.kv_heads > 0x7fffff) return refuse(E_RANGE, "too many tokens or requests in one call");
+    return 0;
+}
+static int attention_plan(aha_paged* p, int heads, int n_tokens, int n, int max_q, int max_len, PagedAttnArgs* a, size_t* bytes) {
+    const aha_paged_desc& d = p->d;
     a->n = n; a->n_tokens = n_tokens; a->max_seqs = d.max_seqs; a->max_blocks = d.max_blocks; a->n_pages = d.n_pages; a->lps = p->lps;
     a->kv_heads = d.kv_heads; a->G = heads / d.kv_heads; a->hd = d.head_dim;
     int cus;
@@ -145,8 +163,9 @@ static int attention_args(aha_paged* p, int heads, int n_tokens, int n, int max_
 }
 extern "C" int aha_paged_attention_workspace(aha_paged* p, int heads, int n_tokens, int n, int max_q, int max_len, size_t* bytes) {
     if (!p || !bytes) return refuse(E_INVAL, "null argument");
+    if (int rc = attention_sizes(p, heads, n_tokens, n, max_q, max_len)) return rc;
     PagedAttnArgs a;
-    return attention_args(p, heads, n_tokens, n, max_q, max_len, &a, bytes);
+    return attention_plan(p, heads, n_tokens, n, max_q, max_len, &a, bytes);
 }
 extern "C" int aha_paged_attention(aha_paged* p, int layer, const void* q, int64_t ldq, int heads, const int32_t* seqs, const int32_t* cu_tokens,
                                    int n, int n_tokens, int max_q, int max_len, int window, float scale, void* out, int64_t ldo, void* workspace,
@@ -156,15 +175,19 @@ extern "C" int aha_paged_attention(aha_paged* p, int layer, const void* q, int64
     if (layer < 0 || layer >= d.layers) return refuse(E_RANGE, "layer out of range");
     if (window < 0) return refuse(E_INVAL, "negative window");
     if (!(scale > 0.f) || scale > 3e38f) return refuse(E_INVAL, "scale must be positive and finite");
-    PagedAttnArgs a;
-    size_t need = 0;
-    if (int rc = attention_args(p, heads, n_tokens, n, max_q, max_len, &a, &need)) return rc;
+    if (int rc = attention_sizes(p, heads, n_tokens, n, max_q, max_len)) return rc;
     if (n_tokens == 0 || n == 0) return 0;
     if (!q || !out || !seqs || !cu_tokens) return refuse(E_INVAL, "null tensor");
     const int64_t qw = (int64_t)heads * d.head_dim;
     if (ldq < qw || ldo < qw || ldq % 8 || ldo % 8) return refuse(E_RANGE, "row strides must hold a row and be multiples of 8 elements");
     if (!aligned16(q) || !aligned16(out) || !aligned16(workspace)) return refuse(E_INVAL, "tensors must be aligned to 16 bytes");
+    if (q == out ? n_tokens > 1 && ldq != ldo : rows_meet(q, ldq, qw, out, ldo, qw, n_tokens))
+        return refuse(E_INVAL, "out overlaps q: it must be q itself, ldq and ldo equal, or lie elsewhere");
+    PagedAttnArgs a;
+    size_t need = 0;
+    if (int rc = attention_plan(p, heads, n_tokens, n, max_q, max_len, &a, &need)) return rc;
     if (need && (!workspace || workspace_bytes < need)) return refuse(E_RANGE, "the workspace has %zu of %zu bytes", workspace_bytes, need);
+    if ((int64_t)window >= (int64_t)d.max_blocks * d.page_size) window = 0;          // no key is that far back
     a.q = (const bf16*)q; a.ldq = ldq; a.out = (bf16*)out; a.ldo = ldo;
     a.k_pages = (char*)d.k_pages + layer * layer_bytes(d); a.v_pages = (char*)d.v_pages + layer * layer_bytes(d);
     a.k_scale = d.k_scale ? d.k_scale + (size_t)layer * d.kv_heads : nullptr;
@@ -173,7 +196,7 @@ extern "C" int aha_paged_attention(aha_paged* p, int layer, const void* q, int64
     a.window = window; a.scale = scale;
     a.part_o = (float*)workspace;
     a.part_ml = need ? a.part_o + paged_partial_floats(&a) : nullptr;
-    a.info = need ? (int*)(a.part_ml + (size_t)a.grid_items * a.kv_heads * a.tile_rows * 2) : nullptr;
+    a.info = need ? (int*)(a.part_ml + (size_t)a.target * a.kv_heads * a.tile_rows * 2) : nullptr;
     RUN("paged attention", paged_attention(&a, d.kv_type == AHA_KV_E4M3, (hipStream_t)st));
     return 0;
 }

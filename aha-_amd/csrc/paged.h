@@ -39,8 +39,8 @@ struct PagedAttnArgs {
     const void *k_pages, *v_pages;               // this layer's
     const float *k_scale, *v_scale;
     const int *table, *lens, *seqs, *cu;
-    float *part_o, *part_ml;                     // [items * kv_heads][tile rows][D] / [..][2]
-    int* info;                                   // [n][2]: a request's first item and its chunks a tile
+    float *part_o, *part_ml;                     // [target][kv_heads][tile rows][D] / [..][2]: partial results
+    int* info;                                   // [n][2]: a request's first partial result and its chunks a tile
     int n, n_tokens, max_seqs, max_blocks, n_pages, lps, kv_heads, G, hd, window;
     float scale;
     int target, min_blocks, cmax;                // the split: see schedule() in paged_attention.hip

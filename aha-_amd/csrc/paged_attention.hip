@@ -24,8 +24,11 @@ typedef const __attribute__((address_space(4))) int* table_t;         // read by
 // longer than S, and none waits for a second round.  The lengths tried are multiples of W / target, W = sum rt_i * nb_i, at least min_blocks; where
 // none is long enough (more tiles than workgroups) the last, under which there are target + (number of tiles) items at most.  Items are
 // numbered request by request, tile by tile.
+//   Only tiles of two chunks or more have partial results, in slots numbered the same way.  There are never more than `target` of them: either all
+// items are no more, or S is at least 2.5 W / target, and C >= 2 means C <= 2 (C - 1) < 2 nb / S, so that they are fewer than 2 W / S = 0.8 target.
+// The workspace therefore does not grow with the tokens (8,192 tokens, 28 / 4 heads of 128: 34 MB, with a slot for each item 154 MB).
 // ---------------------------------------------------------------------------------------------
-struct Work { int req, seq, q0, T, L, first, tile, chunk, chunks; };
+struct Work { int req, seq, q0, T, L, first, slot0, tile, chunk, chunks, slot; };
 
 static __device__ __forceinline__ void request_shape(const PagedAttnArgs& a, int i, int* seq, int* q0, int* T, int* L) {
     *seq = a.seqs[i];
@@ -120,18 +123,19 @@ static __device__ __forceinline__ bool schedule(const PagedAttnArgs& a, int item
     int base = 0;
     Work f;
     if (few) {
-        const int C = chunks_of(a, nb, S), items = me < a.n ? rt * C : 0;
-        const int x = wave_scan(items);
+        const int C = chunks_of(a, nb, S), items = me < a.n ? rt * C : 0, cut = C > 1 ? items : 0;
+        const int x = wave_scan(items), xc = wave_scan(cut);
         const int k = item - (x - items);
         const unsigned long long at = __ballot(k >= 0 && k < items);
         if (!at) return false;
         const int src = __ffsll(at) - 1;
-        f = {src, seq, q0, T, L, item - k, k / C, k % C, C};
+        f = {src, seq, q0, T, L, item - k, xc - cut, k / C, k % C, C, xc - cut + k};
         out->req = src; out->seq = __builtin_amdgcn_readlane(f.seq, src); out->q0 = __builtin_amdgcn_readlane(f.q0, src);
         out->T = __builtin_amdgcn_readlane(f.T, src); out->L = __builtin_amdgcn_readlane(f.L, src); out->first = __builtin_amdgcn_readlane(f.first, src);
         out->tile = __builtin_amdgcn_readlane(f.tile, src); out->chunk = __builtin_amdgcn_readlane(f.chunk, src);
-        out->chunks = __builtin_amdgcn_readlane(f.chunks, src);
+        out->chunks = __builtin_amdgcn_readlane(f.chunks, src); out->slot0 = __builtin_amdgcn_readlane(f.slot0, src); out->slot = __builtin_amdgcn_readlane(f.slot, src);
     } else {
+        int base_cut = 0;
         for (int i0 = 0; i0 < a.n; i0 += NTH) {
             int C = 1, items = 0;
             if (a.n > NTH) {                                // one request a thread: its numbers are still at hand
@@ -139,15 +143,18 @@ static __device__ __forceinline__ bool schedule(const PagedAttnArgs& a, int item
                 if (i0 + tid < a.n) { request_shape(a, i0 + tid, &seq, &q0, &T, &L); request_tiles<TR>(a, T, L, &rt, &nb); }
             }
             if (i0 + tid < a.n) { C = chunks_of(a, nb, S); items = rt * C; }
-            const int x = wave_scan(items);
+            const int cut = C > 1 ? items : 0, x = wave_scan(items), xc = wave_scan(cut);
             __syncthreads();
-            if (lane == 63) isum[0][wave] = x;
+            if (lane == 63) { isum[0][wave] = x; isum[1][wave] = xc; }
             __syncthreads();
-            int before = base;
-            for (int k = 0; k < NTH / 64; ++k) { if (k < wave) before += isum[0][k]; base += isum[0][k]; }
+            int before = base, before_cut = base_cut;
+            for (int k = 0; k < NTH / 64; ++k) {
+                if (k < wave) { before += isum[0][k]; before_cut += isum[1][k]; }
+                base += isum[0][k]; base_cut += isum[1][k];
+            }
             const int k = item - (before + x - items);
             if (k >= 0 && k < items) {
-                found = {i0 + tid, seq, q0, T, L, item - k, k / C, k % C, C};
+                found = {i0 + tid, seq, q0, T, L, item - k, before_cut + xc - cut, k / C, k % C, C, before_cut + xc - cut + k};
                 have = 1;
             }
             __syncthreads();
@@ -159,9 +166,10 @@ static __device__ __forceinline__ bool schedule(const PagedAttnArgs& a, int item
         out->q0 = __builtin_amdgcn_readfirstlane(f.q0); out->T = __builtin_amdgcn_readfirstlane(f.T); out->L = __builtin_amdgcn_readfirstlane(f.L);
         out->first = __builtin_amdgcn_readfirstlane(f.first); out->tile = __builtin_amdgcn_readfirstlane(f.tile);
         out->chunk = __builtin_amdgcn_readfirstlane(f.chunk); out->chunks = __builtin_amdgcn_readfirstlane(f.chunks);
+        out->slot0 = __builtin_amdgcn_readfirstlane(f.slot0); out->slot = __builtin_amdgcn_readfirstlane(f.slot);
     }
     // for the join: where a request's partial results are
-    if (item == out->first && (int)blockIdx.x == item * a.kv_heads && tid == 0 && a.cmax > 1) { a.info[2 * out->req] = out->first; a.info[2 * out->req + 1] = out->chunks; }
+    if (item == out->first && (int)blockIdx.x == item * a.kv_heads && tid == 0 && a.cmax > 1) { a.info[2 * out->req] = out->slot0; a.info[2 * out->req + 1] = out->chunks; }
     return true;
 }
 
@@ -180,9 +188,9 @@ static __device__ __forceinline__ Span tile_span(const PagedAttnArgs& a, const W
 
 // a chunk without keys says so to the join, which then leaves its partial output alone
 template <int TR>
-static __device__ __forceinline__ void no_keys(const PagedAttnArgs& a, int item, int hk) {
+static __device__ __forceinline__ void no_keys(const PagedAttnArgs& a, int slot, int hk) {
     for (int r = threadIdx.x; r < TR; r += blockDim.x) {
-        float* ml = a.part_ml + (((long)item * a.kv_heads + hk) * TR + r) * 2;
+        float* ml = a.part_ml + (((long)slot * a.kv_heads + hk) * TR + r) * 2;
         ml[0] = -INFINITY; ml[1] = 0.f;
     }
 }
@@ -222,7 +230,7 @@ __global__ __launch_bounds__(256) void paged_attn_rows_kernel(PagedAttnArgs a) {
     const int q4 = lane >> 4, r16 = lane & 15;
     const Span sp = tile_span(a, w, w.tile, TR);
     const int b0 = w.chunk * sp.S, b1 = min(sp.nb, b0 + sp.S);
-    if (b0 >= b1 && w.chunks > 1) { no_keys<TR>(a, item, hk); return; }
+    if (b0 >= b1 && w.chunks > 1) { no_keys<TR>(a, w.slot, hk); return; }
     const int R = w.T * a.G, base_pos = w.L - w.T;
 
     // this lane's row and its query
@@ -439,7 +447,7 @@ __global__ __launch_bounds__(256) void paged_attn_rows_kernel(PagedAttnArgs a) {
 #pragma unroll
         for (int e = 0; e < E; ++e) if (c + e < a.hd) op[c + e] = f2bf(acc[e] * inv);
     } else {
-        const long pr = ((long)item * a.kv_heads + hk) * TR + row;
+        const long pr = ((long)w.slot * a.kv_heads + hk) * TR + row;
 #pragma unroll
         for (int e = 0; e < E; ++e) a.part_o[pr * D + c + e] = acc[e];
         if (c == 0) { a.part_ml[pr * 2] = M; a.part_ml[pr * 2 + 1] = lsum; }
@@ -482,7 +490,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
     const int q4 = lane >> 4, r16 = lane & 15;
     const Span sp = tile_span(a, w, w.tile, TR);
     const int b0 = w.chunk * sp.S, b1 = min(sp.nb, b0 + sp.S);
-    if (b0 >= b1 && w.chunks > 1) { no_keys<TR>(a, item, hk); return; }
+    if (b0 >= b1 && w.chunks > 1) { no_keys<TR>(a, w.slot, hk); return; }
     const int R = w.T * a.G, base_pos = w.L - w.T;
     const int row0 = w.tile * TR + wave * 16 * NT;
     const bool wave_on = row0 < R;
@@ -529,17 +537,19 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
     auto no_page = [&](int page) { return (unsigned)page >= (unsigned)a.n_pages; };
     constexpr int NL = E4M3 ? D / 64 : D / 32;              // 16-byte loads a lane of sixteen rows
     u32x4 kreg[NL], vreg[NL];
-    // a lane's byte offsets within sixteen rows: in LDS a row's chunk c lies in place c ^ f(row), so the lane of that place asks for it
+    // a lane's byte offsets within sixteen rows: in LDS a row's chunk c lies in place c ^ f(row), so the lane of that place asks for it; chunks
+    // past the head lie behind the buffer, where a load is zero (a copy of the row's own values could be infinite, and 0 * inf is no zero)
+    auto in_row = [&](int row, int byte) { return byte < row_bytes ? (unsigned)(row * row_bytes + byte) : 0x40000000u; };
     unsigned koff[NL], voff[NL];
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
         if constexpr (!E4M3) {
             const int row = i * LD::RPP + lane / LD::CPR, c = lane % LD::CPR;
-            koff[i] = row * row_bytes + min((LD::k_slot(row, c) - row * D) * 2, row_bytes - 16);
-            voff[i] = row * row_bytes + min((LD::v_slot(row, c) - row * D) * 2, row_bytes - 16);
+            koff[i] = in_row(row, (LD::k_slot(row, c) - row * D) * 2);
+            voff[i] = in_row(row, (LD::v_slot(row, c) - row * D) * 2);
         } else {
             const int idx = i * 64 + lane;
-            koff[i] = voff[i] = idx / (D / 16) * row_bytes + min(idx % (D / 16) * 16, row_bytes - 16);
+            koff[i] = voff[i] = in_row(idx / (D / 16), idx % (D / 16) * 16);
         }
     }
     auto stage = [&](int key0, int page, int buf) {         // wave w has keys 16 w .. 16 w + 15 of a block; bf16: into LDS; e4m3: into registers
@@ -763,7 +773,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
             for (int dt = 0; dt < DT; ++dt)
                 if (dt * 16 < a.hd) *(bf16x4*)(op + dt * 16) = (bf16x4){f2bf(o[nt][dt][0] * inv), f2bf(o[nt][dt][1] * inv), f2bf(o[nt][dt][2] * inv), f2bf(o[nt][dt][3] * inv)};
         } else {
-            const long pr = ((long)item * a.kv_heads + hk) * TR + (wave * NT + nt) * 16 + r16;
+            const long pr = ((long)w.slot * a.kv_heads + hk) * TR + (wave * NT + nt) * 16 + r16;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) *(f32x4*)&a.part_o[pr * D + dt * 16 + 4 * q4] = o[nt][dt];
             if (q4 == 0) { a.part_ml[pr * 2] = m_run[nt]; a.part_ml[pr * 2 + 1] = l; }
@@ -774,7 +784,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
 // ---------------------------------------------------------------------------------------------
 // Joins the chunks of split rows: a wave for each token (of many tokens most have nothing to join), for each token and query head, or, where that
 // leaves the chip empty, four waves for each token and head, which share its chunks.  A lane knows one chunk's maximum and sum, so the weights of
-// 64 chunks take one load; then 64 / (D / 4) partial rows are added at a time.  What bounds it is the chain request -> item -> maximum -> output:
+// 64 chunks take one load; then 64 / (D / 4) partial rows are added at a time.  What bounds it is the chain request -> slot -> maximum -> output:
 // the request is found by counting, not by bisection.
 // ---------------------------------------------------------------------------------------------
 template <int D, int TR, int WAVES>
@@ -800,9 +810,9 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a, i
     const int each = (chunks + WAVES - 1) / WAVES, c_lo = WAVES == 4 ? wave * each : 0, c_hi = min(chunks, c_lo + each);
     for (int h = unit % groups * heads_each, end = h + heads_each; h < end; ++h) {
         const int hk = h / a.G, r = (tok - q0) * a.G + h - hk * a.G, tile = r / TR;
-        const long item = first + (long)(TR > 16 ? rt - 1 - tile : tile) * chunks;         // (the tile kernel takes a request's tiles from the last)
-        if (item < 0 || item + chunks > a.grid_items) return;             // (a cu that is no running sum)
-        const long step = (long)a.kv_heads * TR, p0 = (item * a.kv_heads + hk) * TR + (r - tile * TR);
+        const long slot = first + (long)(TR > 16 ? rt - 1 - tile : tile) * chunks;         // (the tile kernel takes a request's tiles from the last)
+        if (slot < 0 || slot + chunks > a.target) return;             // (a cu that is no running sum)
+        const long step = (long)a.kv_heads * TR, p0 = (slot * a.kv_heads + hk) * TR + (r - tile * TR);
         float M = -INFINITY, l = 0.f;
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
         for (int c0 = c_lo; c0 < c_hi; c0 += 64) {
@@ -871,7 +881,7 @@ static int rows_of_tile(const PagedAttnArgs* a, int max_q) {
 }
 static int template_dim(const PagedAttnArgs* a) { return a->hd <= 64 ? 64 : 128; }
 
-size_t paged_partial_floats(const PagedAttnArgs* a) { return (size_t)a->grid_items * a->kv_heads * a->tile_rows * template_dim(a); }
+size_t paged_partial_floats(const PagedAttnArgs* a) { return (size_t)a->target * a->kv_heads * a->tile_rows * template_dim(a); }
 
 size_t paged_attention_plan(PagedAttnArgs* a, int n_cus, int max_q, int max_len) {
     const int TR = a->tile_rows = rows_of_tile(a, max_q);
@@ -887,7 +897,7 @@ size_t paged_attention_plan(PagedAttnArgs* a, int n_cus, int max_q, int max_len)
     const long by_split = a->target + tiles, by_len = tiles * a->cmax;
     a->grid_items = (int)(by_len < by_split ? by_len : by_split);
     if (a->cmax == 1) return 0;
-    return (paged_partial_floats(a) + (size_t)a->grid_items * a->kv_heads * TR * 2) * sizeof(float) + (size_t)a->n * 2 * sizeof(int);
+    return (paged_partial_floats(a) + (size_t)a->target * a->kv_heads * TR * 2) * sizeof(float) + (size_t)a->n * 2 * sizeof(int);
 }
 
 template <int D, bool E4M3, int TR>

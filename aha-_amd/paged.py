@@ -203,6 +203,8 @@ class PagedKVCache:
             out, _, ldo = self._rows("out", out, heads, out=True)
             if out.shape[0] != N:
                 raise ValueError("out needs as many tokens as q")
+        if window > 0x7fffffff:                                    # (more than a sequence can hold: all keys)
+            window = 0
         key = (heads, N, n, max_q, max_len)
         need = self._workspace.get(key)
         if need is None:                                           # (a function of the sizes alone, asked for once)

@@ -371,16 +371,17 @@ int aha_paged_truncate(aha_paged* p, const int32_t* seqs, const int32_t* new_len
 /* One layer's new tokens: q [n_tokens][heads][head_dim] and k are rotated by the row positions[t] (clamped to 0 .. n_pos-1) of cos / sin (bf16
  * [n_pos][head_dim], the table of aha_ctx_set_rope_table; null: no rotation), q to q_out (may be q), k and v to the pages of their slots; a
  * token with a slot outside the pool is not stored.  Rows have strides ld* in elements (multiples of 8), heads = 0: no queries.  fp32
- * arithmetic, one rounding.  Two tokens of a call must not share a slot. */
+ * arithmetic, one rounding.  Two tokens of a call must not share a slot; q_out may not overlap k, v or, unless it is q, q. */
 int aha_paged_append(aha_paged* p, int layer, const void* q, int64_t ldq, int heads, void* q_out, int64_t ldqo, const void* k, int64_t ldk,
                      const void* v, int64_t ldv, const int32_t* slots, const int32_t* positions, int n_tokens, const void* cos, const void* sin,
                      int n_pos, aha_hip_stream st);
 /* out[t] = softmax(scale * q[t] K^T) V, bf16 [n_tokens][heads][head_dim]: rows cu_tokens[i] .. cu_tokens[i+1]-1 are the LAST tokens of sequence
  * seqs[i] (its keys are already appended) and see the keys at and before their position, the nearest `window` of them (0: all).  heads / kv_heads
- * query heads share a key-value head.  A row that sees no key is 0; rows of padding (negative sequence) and behind cu_tokens[n] are left as
- * they were.  A table entry that is no page hides its keys.  out may be q.  max_q, max_len: the most new tokens and keys of a request (0: not known); they choose the kernel
- * and the split of long sequences, results are right for any value.  workspace: aha_paged_attention_workspace bytes for the same sizes,
- * aligned to 16, used by this call only until its work is done (calls that may run at once need one each). */
+ * query heads share a key-value head.  A row that sees no key, or keys at scores of -infinity only, is 0; rows of padding (negative sequence)
+ * and behind cu_tokens[n] are left as they were.  A table entry that is no page hides its keys.  out may be q, and may not overlap it otherwise.
+ * max_q, max_len: the most new tokens and keys of a request (0: not known); they choose the kernel and the split of long sequences, results
+ * are right for any value.  n_tokens * heads may be at most 2^24 - 1.  workspace: aha_paged_attention_workspace bytes for the same sizes (they do
+ * not grow with n_tokens), aligned to 16, used by this call only until its work is done (calls that may run at once need one each). */
 int aha_paged_attention_workspace(aha_paged* p, int heads, int n_tokens, int n, int max_q, int max_len, size_t* bytes);
 int aha_paged_attention(aha_paged* p, int layer, const void* q, int64_t ldq, int heads, const int32_t* seqs, const int32_t* cu_tokens, int n,
                         int n_tokens, int max_q, int max_len, int window, float scale, void* out, int64_t ldo, void* workspace,

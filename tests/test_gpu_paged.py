@@ -407,6 +407,43 @@ def test_a_value_that_is_not_finite_stays_with_the_rows_that_see_it(T, heads, kv
     assert bool(torch.isnan(got[-1, 0, 3])) and not bool(torch.isnan(got[0].float()).any())
 
 
+@pytest.mark.parametrize("dim", [80, 128])
+@pytest.mark.parametrize("T", [1, 3, 40, 140])
+def test_a_key_at_minus_infinity_weighs_nothing(T, dim):
+    """As one at a score so low that its exponential is zero, bit for bit; also where the head is narrower than the kernel's tiles."""
+    c = filled([300], 16, 4, 2, dim, "bf16", 13)
+    q = randn(gen(14), T, 4, dim).bfloat16()
+    q[..., dim - 1] = 1.0
+    for j in (5, 100, 299 - T // 2):
+        c.k_pages[0, int(c.block_table[0, j // 16]), :, j % 16, dim - 1] = -1e5
+    seqs, cu = ints([0]), ints([0, T])
+    want = check_attention(c, q, seqs, cu, max_q=T, max_len=300)
+    c.k_pages[c.k_pages == c.k_pages.new_tensor(-1e5)] = float("-inf")
+    assert bool(torch.isinf(c.k_pages).any())
+    assert torch.equal(c.attention(0, q, seqs, cu, max_q=T, max_len=300), want)
+
+
+@pytest.mark.parametrize("T", [1, 20])
+def test_a_window_beyond_every_length_is_none(T):
+    c = filled([5, 400], 16, 4, 2, 64, "bf16", 15)
+    q = randn(gen(16), 2 * T, 4, 64).bfloat16()
+    seqs, cu = ints([0, 1]), ints([0, T, 2 * T])                             # (more rows than the first has keys: they are zero)
+    want = check_attention(c, q, seqs, cu, max_q=T)
+    for window in (c.max_blocks * c.page_size, 2 ** 31 - 1, 2 ** 31, 2 ** 40 + 1):
+        assert torch.equal(c.attention(0, q, seqs, cu, max_q=T, window=window), want)
+
+
+def test_the_workspace_does_not_grow_with_the_tokens():
+    import ctypes as C
+    c = filled([100], 16, 28, 4, 128, "bf16", 25)
+    need = []
+    for tokens in (2048, 16384, 131072):
+        b = C.c_size_t()
+        c._chk(c.lib.aha_paged_attention_workspace(c.handle, 28, tokens, 1, tokens, 0, C.byref(b)))
+        need.append(b.value)
+    assert need[0] == need[1] == need[2]
+
+
 def test_attention_scale_strides_and_sharp_rows():
     """Rows of a fused projection in, strided rows out; a query that puts all its weight on one key returns that key's value."""
     c = filled([500], 64, 14, 2, 128, "bf16", 21, rubbish=False)

@@ -131,6 +131,26 @@ def test_attention_refuses(monkeypatch):
     assert c.lib.aha_paged_attention_workspace(c.handle, 4, 3, 2, 1, 1, None) == -22
 
 
+def test_outputs_that_overlap_inputs_are_refused(monkeypatch):
+    """In place is fine, and so are columns of one buffer; anything else that shares an element is not."""
+    monkeypatch.setattr(PagedKVCache, "_stream", lambda self: 0)
+    c = make()
+    buf = torch.zeros((8, 256), dtype=torch.bfloat16)
+    q, k, v, s = buf[:3, :128], buf[:3, 128:192], buf[:3, 192:], torch.zeros(3, dtype=I)
+    call, lib, p = c.lib.aha_paged_attention, c.lib, s.data_ptr()
+
+    def attend(out):
+        return call(c.handle, 0, q.data_ptr(), 256, 4, p, p, 1, 3, 1, 16, 0, 0.1, out.data_ptr(), out.stride(0), p, 0, None)
+
+    flat = buf.view(-1)
+    for out in (buf[1:4, :128], buf[:3, 64:192], buf[:3, 8:136], flat[:3 * 128].view(3, 128), flat[256:256 + 3 * 128].view(3, 128)):
+        with pytest.raises(AhaError, match="overlaps"):
+            c.append(0, q, k, v, s, q_out=out)
+        assert attend(out) == -22 and b"out overlaps q" in lib.aha_paged_last_error()
+    with pytest.raises(AhaError, match="overlaps k or v"):
+        c.append(0, torch.zeros((3, 128), dtype=torch.bfloat16), k, v, s, q_out=buf[:3, 96:224])
+
+
 def test_no_cpu_fallback_and_no_gradient():
     c = make()
     seqs, counts = torch.zeros(2, dtype=I), torch.ones(2, dtype=I)
