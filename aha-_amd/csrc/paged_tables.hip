@@ -9,7 +9,8 @@
 // One workgroup does a call: the work is a prefix sum over the requests and a few words per page and token, and what bounds it is the chain
 // sequence -> length -> sum -> free entry -> store, each link a trip to the L2 or memory.  All requests are looked at before anything is
 // written, so a call that cannot be done (status) changes nothing.  Pages and tokens are dealt out flat, a thread finds the request of its
-// page or token by bisection of the sums in LDS: a request of two thousand tokens does not keep one thread busy.
+// page or token by bisection of the sums in LDS: a request of two thousand tokens does not keep one thread busy.  16 requests of a token: reserve
+// 4.2 us, truncate 3.0; 256 of some 250 tokens (64,700): 7.0 and 4.0 for the slots, truncate 5.9.
 #include "paged.h"
 
 struct Scan2 { int a, b; };
