@@ -28,7 +28,8 @@ _TYPES = {torch.bfloat16: _l.KV_BF16, torch.float8_e4m3fn: _l.KV_E4M3}
 
 
 class PagedKVCache:
-    """One pool.  `rope`: (cos, sin), bf16 [positions, head_dim], what `append` rotates with; without it keys and queries come rotated.
+    """One pool.  `rope`: (cos, sin), bf16 [positions, head_dim], what `append` rotates with
+    (positions behind its last as the last); without it keys and queries come rotated.
     `k_scale` / `v_scale`: fp32 [layers, kv_heads] of an e4m3 pool (default 1).  The tensors (`k_pages`, `v_pages`: [layers, n_pages, kv_heads,
     page_size, head_dim]; `block_table` [max_seqs, max_blocks], `lens` [max_seqs], `free_pages` [n_pages], `n_free` [1], all int32) are made
     here unless given, and are the caller's to look at; pages may hold anything."""

@@ -513,6 +513,24 @@ def test_many_requests():
     check_attention(c, q, ints(order), cu, max_q=3, max_len=3000)
 
 
+@pytest.mark.parametrize("n,T", [(100, 1), (100, 20), (300, 1), (300, 40)])
+def test_many_requests_of_which_some_are_cut(n, T):
+    """Short requests between long ones: the partial results of the cut ones lie one behind the other."""
+    lens = [40 + i % 7 for i in range(n)]
+    for i in (0, 63, 64, n // 2, n - 1):
+        lens[i] = 5000 + 777 * (i % 3)
+    c = filled(lens, 64, 4, 2, 64, "bf16", 33)
+    q = randn(gen(34), n * T, 4, 64).bfloat16()
+    got = check_attention(c, q, ints(range(n)), ints(range(0, n * T + 1, T)), max_q=T)
+    assert torch.equal(c.attention(0, q, ints(range(n)), ints(range(0, n * T + 1, T)), max_q=T), got)
+
+
+def test_one_token_over_as_many_chunks_as_workgroups():
+    c = filled([80000], 128, 8, 1, 64, "bf16", 35)
+    check_attention(c, randn(gen(36), 1, 8, 64).bfloat16(), ints([0]), ints([0, 1]), max_q=1)
+    check_attention(c, randn(gen(37), 3, 8, 64).bfloat16(), ints([0]), ints([0, 3]), max_q=3)
+
+
 @pytest.mark.parametrize("T,L,kind", [(1, 30001, "bf16"), (1, 20000, "e4m3"), (5, 9000, "bf16"), (36, 6000, "bf16"), (700, 1500, "e4m3")])
 def test_long_sequences_and_the_same_bits_twice(T, L, kind):
     c = filled([L, 40], 64, 28, 4, 128, kind, L)
