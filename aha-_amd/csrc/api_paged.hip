@@ -194,6 +194,7 @@ extern "C" int aha_paged_attention(aha_paged* p, int layer, const void* q, int64
     a.v_scale = d.v_scale ? d.v_scale + (size_t)layer * d.kv_heads : nullptr;
     a.table = d.block_table; a.lens = d.lens; a.seqs = seqs; a.cu = cu_tokens;
     a.window = window; a.scale = scale;
+    a.most_keys = window && window < 0x7fffffff - a.tile_rows - 65 ? window + a.tile_rows / a.G + 65 : 0x7fffffff;
     a.part_o = (float*)workspace;
     a.part_ml = need ? a.part_o + paged_partial_floats(&a) : nullptr;
     a.info = need ? (int*)(a.part_ml + (size_t)a.target * a.kv_heads * a.tile_rows * 2) : nullptr;

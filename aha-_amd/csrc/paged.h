@@ -34,6 +34,8 @@ struct PagedAppendArgs {
     int n_tokens, heads, kv_heads, hd, lps, n_slots, e4m3;
 };
 
+struct PagedDiv { unsigned mul; int shift; };     // n / d = (high word of n * mul, + n) >> shift
+
 struct PagedAttnArgs {
     const bf16* q; long ldq; bf16* out; long ldo;
     const void *k_pages, *v_pages;               // this layer's
@@ -44,6 +46,9 @@ struct PagedAttnArgs {
     int n, n_tokens, max_seqs, max_blocks, n_pages, lps, kv_heads, G, hd, window;
     float scale;
     int target, min_blocks, cmax;                // the split: see schedule() in paged_attention.hip
+    float inv_target;
+    int most_keys;                               // that a tile's rows see between them
+    PagedDiv by_G, by_kv_heads, by_heads;
     int grid_items, tile_rows;                   // workgroups a key-value head; rows of a tile
 };
 

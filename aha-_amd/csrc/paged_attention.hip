@@ -43,14 +43,15 @@ static __device__ __forceinline__ void request_shape(const PagedAttnArgs& a, int
 }
 template <int TR>
 static __device__ __forceinline__ void request_tiles(const PagedAttnArgs& a, int T, int L, int* rt, int* nb) {
-    *rt = (int)(((long)T * a.G + TR - 1) / TR);
-    int keys = L;
-    if (a.window) keys = (int)min((long)keys, (long)a.window + TR / a.G + 65);
-    *nb = (keys + 63) >> 6;
+    *rt = (T * a.G + TR - 1) / TR;
+    *nb = (min(L, a.most_keys) + 63) >> 6;
 }
-static __device__ __forceinline__ int chunks_of(const PagedAttnArgs& a, int nb, float S) {
-    return min(max((int)ceilf((float)nb / S - 1e-3f), 1), a.cmax);
+// (nb / S is W / S at most, so the error of a reciprocal is far below the 1e-3)
+static __device__ __forceinline__ int chunks_of(const PagedAttnArgs& a, int nb, float inv_S) {
+    return min(max((int)ceilf(__builtin_fmaf((float)nb, inv_S, -1e-3f)), 1), a.cmax);
 }
+// n / d for 0 <= n < 2^31
+static __device__ __forceinline__ int quot(int n, PagedDiv d) { return (int)((__umulhi((unsigned)n, d.mul) + (unsigned)n) >> d.shift); }
 // running sum over the wave's lanes (data-parallel moves: no trip through LDS); the last lane has the total
 template <class T>
 static __device__ __forceinline__ T wave_scan(T x) {
@@ -99,17 +100,21 @@ static __device__ __forceinline__ bool schedule(const PagedAttnArgs& a, int item
 #pragma unroll
         for (int k = 0; k < NTH / 64; ++k) W += fsum[k];
     }
-    const float S0 = W / (float)a.target;
-    int cnt[TRIES];
+    const float S0 = W * a.inv_target, least = (float)a.min_blocks;
+    int cnt[TRIES];                                         // up to 1,023 a lane: two counts of 64 lanes in a word, and more than `target`
+    float inv_S[TRIES];
 #pragma unroll
-    for (int k = 0; k < TRIES; ++k) cnt[k] = 0;
+    for (int k = 0; k < TRIES; ++k) { cnt[k] = 0; inv_S[k] = __builtin_amdgcn_rcpf(fmaxf(least, S0 * tries[k])); }
     for (int i = me; i < a.n; i += step) {
         if (a.n > step) { request_shape(a, i, &seq, &q0, &T, &L); request_tiles<TR>(a, T, L, &rt, &nb); }
 #pragma unroll
-        for (int k = 0; k < TRIES; ++k) cnt[k] += rt * chunks_of(a, nb, fmaxf((float)a.min_blocks, S0 * tries[k]));
+        for (int k = 0; k < TRIES; ++k) cnt[k] = min(cnt[k] + rt * chunks_of(a, nb, inv_S[k]), 1023);
     }
 #pragma unroll
-    for (int k = 0; k < TRIES; ++k) cnt[k] = wave_total(cnt[k]);
+    for (int k = 0; k < TRIES; k += 2) {
+        const unsigned both = (unsigned)wave_total(cnt[k] | cnt[k + 1] << 16);
+        cnt[k] = both & 0xffff; cnt[k + 1] = both >> 16;
+    }
     if (!few) {
         if (lane == 0)
 #pragma unroll
@@ -122,11 +127,10 @@ static __device__ __forceinline__ bool schedule(const PagedAttnArgs& a, int item
             for (int x = 0; x < NTH / 64; ++x) cnt[k] += isum[k][x];
         }
     }
-    float S = S0 * tries[TRIES - 1];
+    float S = inv_S[TRIES - 1];                             // (its reciprocal)
 #pragma unroll
     for (int k = TRIES - 2; k >= 0; --k)
-        if (cnt[k] <= a.target) S = S0 * tries[k];
-    S = fmaxf(S, (float)a.min_blocks);
+        if (cnt[k] <= a.target) S = inv_S[k];
     int base = 0;
     Work f;
     if (few) {
@@ -136,7 +140,8 @@ static __device__ __forceinline__ bool schedule(const PagedAttnArgs& a, int item
         const unsigned long long at = __ballot(k >= 0 && k < items);
         if (!at) return false;
         const int src = __ffsll(at) - 1;
-        f = {src, seq, q0, T, L, item - k, xc - cut, k / C, k % C, C, xc - cut + k};
+        const int tile = (int)((unsigned)(k & 0xffffff) / (unsigned)(C & 0xffff));
+        f = {src, seq, q0, T, L, item - k, xc - cut, tile, k - tile * C, C, xc - cut + k};
         out->req = src; out->seq = __builtin_amdgcn_readlane(f.seq, src); out->q0 = __builtin_amdgcn_readlane(f.q0, src);
         out->T = __builtin_amdgcn_readlane(f.T, src); out->L = __builtin_amdgcn_readlane(f.L, src); out->first = __builtin_amdgcn_readlane(f.first, src);
         out->tile = __builtin_amdgcn_readlane(f.tile, src); out->chunk = __builtin_amdgcn_readlane(f.chunk, src);
@@ -184,7 +189,7 @@ static __device__ __forceinline__ bool schedule(const PagedAttnArgs& a, int item
 struct Span { int lo, hi, first, nb, S; };
 static __device__ __forceinline__ Span tile_span(const PagedAttnArgs& a, const Work& w, int tile, int TR) {
     Span s;
-    const int t0 = tile * TR / a.G, t1 = min((tile * TR + TR - 1) / a.G, w.T - 1);
+    const int t0 = quot(tile * TR, a.by_G), t1 = min(quot(tile * TR + TR - 1, a.by_G), w.T - 1);
     s.hi = max(0, min(w.L, w.L - w.T + t1 + 1));
     s.lo = a.window ? max(0, w.L - w.T + t0 + 1 - a.window) : 0;
     s.first = s.lo & ~63;
@@ -220,7 +225,7 @@ static __device__ __forceinline__ bf16x8 e4m3x8(unsigned lo, unsigned hi) {     
 // Few rows (one token: the G rows of a key-value head): bound by the bytes of K and V.  A workgroup's four waves take blocks of 32 keys in turn,
 // each with a softmax of its own and no barrier in the loop, and are merged at the end.  The matrix cores have time to spare, so P goes into
 // the product as two bf16 halves (high and remainder): no precision is lost to its rounding (2^-17 of p).  28 / 4 heads of 128: 16 tokens over
-// 12,000 keys each (393 MB) 72 us, 5.4 TB/s; 64 over 9,000 in e4m3 (590 MB) 109 us, 5.4 TB/s (a large copy: 4.9).  One over 2,048 keys 8.2 us: the
+// 12,000 keys each (393 MB) 72 us, 5.4 TB/s; 64 over 9,000 in e4m3 (590 MB) 109 us, 5.4 TB/s (a large copy: 4.9).  One over 2,048 keys 7.2 us: the
 // chain of request, length, table, keys, merge, each link a trip to memory.
 // ---------------------------------------------------------------------------------------------
 template <int D, bool E4M3>
@@ -232,7 +237,7 @@ __global__ __launch_bounds__(256) void paged_attn_rows_kernel(PagedAttnArgs a) {
     __shared__ __attribute__((aligned(16))) bf16 Vs[4][32 * VST];
     __shared__ float sm[4][16], sl[4][16];
 
-    const int item = blockIdx.x / a.kv_heads, hk = blockIdx.x - item * a.kv_heads;
+    const int item = quot(blockIdx.x, a.by_kv_heads), hk = blockIdx.x - item * a.kv_heads;
     Work w;
     if (!schedule<256, TR>(a, item, &w)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -244,7 +249,7 @@ __global__ __launch_bounds__(256) void paged_attn_rows_kernel(PagedAttnArgs a) {
 
     // this lane's row and its query
     bf16x8 qf[KSQ];
-    const int my_r = min(w.tile * TR + r16, R - 1), my_t = my_r / a.G, pos = base_pos + my_t;
+    const int my_r = min(w.tile * TR + r16, R - 1), my_t = quot(my_r, a.by_G), pos = base_pos + my_t;
     {
         const bf16* qp = a.q + (long)(w.q0 + my_t) * a.ldq + (long)(hk * a.G + my_r - my_t * a.G) * a.hd;
         const bf16x8 z8 = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -256,7 +261,7 @@ __global__ __launch_bounds__(256) void paged_attn_rows_kernel(PagedAttnArgs a) {
             qf[ks] = ch < a.hd ? v : z8;
         }
     }
-    const int pos_min = base_pos + w.tile * TR / a.G, pos_max = base_pos + min((w.tile * TR + TR - 1) / a.G, w.T - 1);
+    const int pos_min = base_pos + quot(w.tile * TR, a.by_G), pos_max = base_pos + min(quot(w.tile * TR + TR - 1, a.by_G), w.T - 1);
     const bool one_pos = pos_min == pos_max;
     const float c2 = a.scale * (E4M3 && a.k_scale ? a.k_scale[hk] : 1.f) * 1.4426950408889634f;
 
@@ -451,7 +456,7 @@ __global__ __launch_bounds__(256) void paged_attn_rows_kernel(PagedAttnArgs a) {
     if (w.chunks == 1) {
         // a row that sees no key is zero; NaN stays
         const float inv = lsum > 0.f ? (E4M3 && a.v_scale ? a.v_scale[hk] : 1.f) / lsum : lsum == 0.f ? 0.f : lsum;
-        const int t = r / a.G;
+        const int t = quot(r, a.by_G);
         bf16* op = a.out + (long)(w.q0 + t) * a.ldo + (long)(hk * a.G + r - t * a.G) * a.hd;
 #pragma unroll
         for (int e = 0; e < E; ++e) if (c + e < a.hd) op[c + e] = f2bf(acc[e] * inv);
@@ -494,10 +499,10 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
     extern __shared__ __attribute__((aligned(16))) bf16 kv[];             // [buffer][K, V][64][D]
     __shared__ int odd_s[2];
 
-    const int item = blockIdx.x / a.kv_heads, hk = blockIdx.x - item * a.kv_heads;
+    const int item = quot(blockIdx.x, a.by_kv_heads), hk = blockIdx.x - item * a.kv_heads;
     Work w;
     if (!schedule<256, TR>(a, item, &w)) return;
-    w.tile = (int)(((long)w.T * a.G + TR - 1) / TR) - 1 - w.tile;         // the longest rows of a prompt first
+    w.tile = (w.T * a.G + TR - 1) / TR - 1 - w.tile;         // the longest rows of a prompt first
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int q4 = lane >> 4, r16 = lane & 15;
     const Span sp = tile_span(a, w, w.tile, TR);
@@ -511,7 +516,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
     bf16x8 qf[NT][KSQ];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const int r = min(row0 + nt * 16 + r16, R - 1), t = r / a.G, g = r - t * a.G;
+        const int r = min(row0 + nt * 16 + r16, R - 1), t = quot(r, a.by_G), g = r - t * a.G;
         pos[nt] = base_pos + t;
         const bf16* qp = a.q + (long)(w.q0 + t) * a.ldq + (long)(hk * a.G + g) * a.hd;
         const bf16x8 z8 = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -523,8 +528,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
         }
     }
     // the positions of the workgroup's rows, and of the wave's
-    const int pos_lo = base_pos + w.tile * TR / a.G, pos_hi = base_pos + min((w.tile * TR + TR - 1) / a.G, w.T - 1);
-    const int wpos_lo = base_pos + min(row0, R - 1) / a.G, wpos_hi = base_pos + min(row0 + 16 * NT - 1, R - 1) / a.G;
+    const int pos_lo = base_pos + quot(w.tile * TR, a.by_G), pos_hi = base_pos + min(quot(w.tile * TR + TR - 1, a.by_G), w.T - 1);
+    const int wpos_lo = base_pos + quot(min(row0, R - 1), a.by_G), wpos_hi = base_pos + quot(min(row0 + 16 * NT - 1, R - 1), a.by_G);
     const float c2 = a.scale * (E4M3 && a.k_scale ? a.k_scale[hk] : 1.f) * 1.4426950408889634f;
 
     f32x4 o[NT][DT], lacc[NT];
@@ -779,7 +784,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
         const float l = lacc[nt][0];
         if (w.chunks == 1) {
             const float inv = l > 0.f ? vsc / l : l == 0.f ? 0.f : l;
-            const int t = r / a.G, g = r - t * a.G;
+            const int t = quot(r, a.by_G), g = r - t * a.G;
             bf16* op = a.out + (long)(w.q0 + t) * a.ldo + (long)(hk * a.G + g) * a.hd + 4 * q4;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
@@ -805,9 +810,9 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a, i
     constexpr int LPR = D / 4, AT = 64 / LPR, FLY = WAVES == 4 ? 8 : 4;   // lanes of a row, rows at a time, loads under way
     __shared__ float sh_m[4], sh_l[4];
     __shared__ f32x4 sh_o[4][LPR];
-    const int heads = a.kv_heads * a.G, groups = heads / heads_each, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int heads = a.kv_heads * a.G, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int unit = WAVES == 4 ? blockIdx.x : blockIdx.x * 4 + wave, lane = threadIdx.x & 63;
-    const int tok = unit / groups;
+    const int tok = heads_each == 1 ? quot(unit, a.by_heads) : unit, h0 = heads_each == 1 ? unit - tok * heads : 0;    // (one head or all)
     if (tok >= a.n_tokens) return;
     int req = 0;
     if (a.n <= 512) {
@@ -817,12 +822,12 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a, i
         while (req < hi) { const int mid = (req + hi) >> 1; if (a.cu[mid + 1] <= tok) req = mid + 1; else hi = mid; }
     }
     if (req >= a.n) return;                                 // behind the last request
-    const int q0 = a.cu[req], T = a.cu[req + 1] - q0, seq = a.seqs[req], first = a.info[2 * req], chunks = a.info[2 * req + 1];
+    const int q0 = min(max(a.cu[req], 0), a.n_tokens), T = min(max(a.cu[req + 1], q0), a.n_tokens) - q0, seq = a.seqs[req], first = a.info[2 * req], chunks = a.info[2 * req + 1];
     if (tok < q0 || (unsigned)seq >= (unsigned)a.max_seqs || chunks <= 1) return;
-    const int rt = (int)(((long)T * a.G + TR - 1) / TR), col = lane % LPR * 4, sub = lane / LPR;
+    const int rt = (T * a.G + TR - 1) / TR, col = lane % LPR * 4, sub = lane / LPR;
     const int each = (chunks + WAVES - 1) / WAVES, c_lo = WAVES == 4 ? wave * each : 0, c_hi = min(chunks, c_lo + each);
-    for (int h = unit % groups * heads_each, end = h + heads_each; h < end; ++h) {
-        const int hk = h / a.G, r = (tok - q0) * a.G + h - hk * a.G, tile = r / TR;
+    for (int h = h0; h < h0 + heads_each; ++h) {
+        const int hk = quot(h, a.by_G), r = (tok - q0) * a.G + h - hk * a.G, tile = r / TR;
         const long slot = first + (long)(TR > 16 ? rt - 1 - tile : tile) * chunks;         // (the tile kernel takes a request's tiles from the last)
         if (slot < 0 || slot + chunks > a.target) return;             // (a cu that is no running sum)
         const long step = (long)a.kv_heads * TR, p0 = (slot * a.kv_heads + hk) * TR + (r - tile * TR);
@@ -902,12 +907,21 @@ static int template_dim(const PagedAttnArgs* a) { return a->hd <= 64 ? 64 : 128;
 
 size_t paged_partial_floats(const PagedAttnArgs* a) { return (size_t)a->target * a->kv_heads * a->tile_rows * template_dim(a); }
 
+static PagedDiv div_by(unsigned d) {
+    int s = 0;
+    while ((1u << s) < d) ++s;
+    return {(unsigned)(((uint64_t)1 << 32) * (((uint64_t)1 << s) - d) / d + 1), s};
+}
+
 size_t paged_attention_plan(PagedAttnArgs* a, int n_cus, int max_q, int max_len) {
     const int TR = a->tile_rows = rows_of_tile(a, max_q);
     const long tiles = (long)a->n_tokens * a->G / TR + a->n;              // of one key-value head, at most
     // Two workgroups a CU: what registers and LDS let run at once, and fewer, longer ones leave less to join (four, for tokens, against two:
     // sixteen over 12,000 keys 80.7 / 77.9 us, one over 32,000 29.3 / 22.7 us).
     a->target = (2 * n_cus + a->kv_heads - 1) / a->kv_heads;
+    if (a->target > 1000) a->target = 1000;                               // (see TRIES)
+    a->inv_target = 1.f / (float)a->target;
+    a->by_G = div_by(a->G); a->by_kv_heads = div_by(a->kv_heads); a->by_heads = div_by(a->G * a->kv_heads);
     a->min_blocks = 2;                                                    // 128 keys: a block of 32 for each of four waves (64 keys at least: within 2 % either way)
     long cap = (long)a->max_blocks << a->lps;
     if (max_len > 0 && max_len < cap) cap = max_len;
