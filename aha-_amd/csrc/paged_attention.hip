@@ -926,7 +926,11 @@ size_t paged_attention_plan(PagedAttnArgs* a, int n_cus, int max_q, int max_len)
     long cap = (long)a->max_blocks << a->lps;
     if (max_len > 0 && max_len < cap) cap = max_len;
     const long nb = (cap + 63) / 64;
-    a->cmax = (int)(nb / a->min_blocks < 1 ? 1 : nb / a->min_blocks);
+    // Short sequences are not split, which saves the join and its launch, twice as far where tiles fill half the CUs anyway; us split / whole, heads
+    // of 128: one token over 512 keys 13.6 / 11.1, 768 12.8 / 14.0; 64 tokens over 1,024 keys 28.5 / 24.8; 5 over 384 12.9 / 12.2, over 512 12.9 / 14.2;
+    // 16 x 36 over 384 27 / 18, one of 40, heads of 64, over 768 13.3 / 18.2; tokens with heads of 64: one over 768 12.7 / 10.4, 128 over 2,048 30 / 23.8.
+    const long whole = (TR > 16 ? 6 : a->hd > 64 ? 8 : 16) * (2 * tiles * a->kv_heads >= n_cus ? 2 : 1);
+    a->cmax = (int)(nb <= whole ? 1 : nb / a->min_blocks);
     const long by_split = a->target + tiles, by_len = tiles * a->cmax;
     a->grid_items = (int)(by_len < by_split ? by_len : by_split);
     if (a->cmax == 1) return 0;
