@@ -4,7 +4,8 @@
 //           requests' needs, summed in order, say which entries of the free list they take, counted from its end.  Token t of request i
 //           has position len_i + t and slot page(position / P) * P + position % P.
 // truncate: the pages behind the first ceil(new_len / P) go back to the free list, in the order in which a reserve of the same requests
-//           takes them: a truncate to the old lengths leaves the list as it was before the reserve, entry by entry.
+//           takes them: a truncate to the old lengths leaves the list as it was before the reserve, entry by entry.  A table entry that is no
+//           page (attention lets callers drop the pages before a window) has nothing to give back: it is passed over, never put on the list.
 //
 // One workgroup does a call: the work is a prefix sum over the requests and a few words per page and token, and what bounds it is the chain
 // sequence -> length -> sum -> free entry -> store, each link a trip to the L2 or memory.  All requests are looked at before anything is
@@ -83,13 +84,13 @@ __global__ __launch_bounds__(PT_THREADS) void paged_tables_kernel(PagedReserveAr
     __shared__ unsigned seen[PAGED_MAX_SEQS / 32];
     __shared__ Scan2 wsum[PT_THREADS / 64];
     __shared__ int pend[PT_THREADS], tend[PT_THREADS], rseq[PT_THREADS], rhad[PT_THREADS], rlen[PT_THREADS];
-    __shared__ int err_s;
+    __shared__ int err_s, good_s;
     __shared__ unsigned long long pages_s, tokens_s;
     const int tid = threadIdx.x, NT = blockDim.x;
     const PagedTables& t = a.t;
     const int words = (t.max_seqs + 31) >> 5;
     for (int i = tid; i < words; i += NT) seen[i] = 0;
-    if (tid == 0) { err_s = 0; pages_s = 0; tokens_s = 0; }
+    if (tid == 0) { err_s = 0; good_s = 0; pages_s = 0; tokens_s = 0; }
     const int n_free = min(max(*t.n_free, 0), t.n_pages);
     Request r0 = look<RESERVE>(a, tid);                        // kept: with at most NT requests nothing is read twice
     __syncthreads();
@@ -113,11 +114,32 @@ __global__ __launch_bounds__(PT_THREADS) void paged_tables_kernel(PagedReserveAr
     __syncthreads();
     err = err_s; pages = pages_s; tokens = tokens_s;
     unsigned long long missing = 0;
+    int gone = 0;                                              // truncate: pages that go back
+    Scan2 all = {0, 0};
     if (err) {                                                 // the sums of requests that are none say nothing
     } else if (RESERVE) {
         if (pages > (unsigned long long)n_free) { err |= PAGED_NO_PAGES; missing = pages - n_free; }
         if (tokens > (unsigned long long)a.n_tokens) err |= PAGED_MANY_TOKENS;
-    } else if (pages + n_free > (unsigned long long)t.n_pages) err |= PAGED_BAD_SEQ;       // more pages than the pool has: the tables are not its own
+    } else if (pages > 0x7fffffffull - 4096) err |= PAGED_BAD_SEQ;          // (more than the sums below hold: no table has as many)
+    else {
+        // only entries that are pages go back: how many are there?
+        int good = 0;
+        for (int i0 = 0; i0 < a.n; i0 += NT) {
+            const Request r = i0 ? look<RESERVE>(a, i0 + tid) : r0;
+            pend[tid] = block_scan({r.need, 0}, wsum, &all).a; rseq[tid] = r.seq; rhad[tid] = r.had;
+            __syncthreads();
+            const int m = min(NT, a.n - i0);
+            for (int p = tid; p < all.a; p += NT) {
+                const int i = bisect(pend, m, p);
+                good += (unsigned)t.table[(long)rseq[i] * t.max_blocks + rhad[i] + p - (i ? pend[i - 1] : 0)] < (unsigned)t.n_pages;
+            }
+            __syncthreads();
+        }
+        if (good) atomicAdd(&good_s, good);
+        __syncthreads();
+        gone = good_s;
+        if ((long)gone + n_free > t.n_pages) err |= PAGED_BAD_SEQ;       // more pages than the pool has: the tables are not its own
+    }
     if (tid == 0) {
         a.status[0] = err;
         a.status[1] = missing > 0x7fffffffull ? 0x7fffffff : (int)missing;
@@ -131,24 +153,41 @@ __global__ __launch_bounds__(PT_THREADS) void paged_tables_kernel(PagedReserveAr
     }
 
     // ---- deal out pages and tokens
-    Scan2 base = {0, 0};
+    Scan2 base = {0, 0};                                       // (truncate: of entries; `back` of pages among them)
+    int back = 0;
     for (int i0 = 0; i0 < a.n; i0 += NT) {
         const Request r = i0 ? look<RESERVE>(a, i0 + tid) : r0;
-        Scan2 all;
-        const Scan2 in = block_scan({r.need, RESERVE ? r.count : 0}, wsum, &all);
-        pend[tid] = in.a; tend[tid] = in.b; rseq[tid] = r.seq; rhad[tid] = r.had; rlen[tid] = r.len;
-        if (RESERVE && i0 + tid < a.n) {
-            a.cu[i0 + tid + 1] = base.b + in.b;
-            if (i0 + tid == 0) a.cu[0] = 0;
+        if (RESERVE || a.n > NT) {                             // (else the count has left the sums as they are needed)
+            const Scan2 in = block_scan({r.need, RESERVE ? r.count : 0}, wsum, &all);
+            pend[tid] = in.a; tend[tid] = in.b; rseq[tid] = r.seq; rhad[tid] = r.had; rlen[tid] = r.len;
+            if (RESERVE && i0 + tid < a.n) {
+                a.cu[i0 + tid + 1] = base.b + in.b;
+                if (i0 + tid == 0) a.cu[0] = 0;
+            }
+            __syncthreads();
         }
-        __syncthreads();
         const int m = min(NT, a.n - i0);
-        for (int p = tid; p < all.a; p += NT) {
-            const int i = bisect(pend, m, p);
-            const int k = p - (i ? pend[i - 1] : 0);
-            int* e = t.table + (long)rseq[i] * t.max_blocks + rhad[i] + k;
-            if (RESERVE) *e = t.free_pages[n_free - 1 - (base.a + p)];
-            else { t.free_pages[n_free + (int)pages - 1 - (base.a + p)] = *e; *e = -1; }
+        const bool whole = (unsigned long long)gone == pages;  // every entry is a page: the p-th entry is the p-th page
+        for (int p0 = 0; p0 < all.a; p0 += NT) {
+            const int p = p0 + tid;
+            int* e = nullptr;
+            if (p < all.a) {
+                const int i = bisect(pend, m, p);
+                e = t.table + (long)rseq[i] * t.max_blocks + rhad[i] + p - (i ? pend[i - 1] : 0);
+            }
+            if (RESERVE) {
+                if (e) *e = t.free_pages[n_free - 1 - (base.a + p)];
+            } else {
+                const int page = e ? *e : -1, good = (unsigned)page < (unsigned)t.n_pages;
+                int at = base.a + p;
+                if (!whole) {
+                    Scan2 here;
+                    at = back + block_scan({good, 0}, wsum, &here).a - good;
+                    back += here.a;
+                }
+                if (good) t.free_pages[n_free + gone - 1 - at] = page;
+                if (e) *e = -1;
+            }
         }
         if (RESERVE && map_tokens)
             for (int x = tid; x < all.b; x += NT) {
@@ -166,7 +205,7 @@ __global__ __launch_bounds__(PT_THREADS) void paged_tables_kernel(PagedReserveAr
     if (RESERVE && map_tokens)
         for (int x = base.b + tid; x < a.n_tokens; x += NT) { a.slots[x] = -1; a.positions[x] = -1; }
     if (RESERVE && a.n == 0 && tid == 0) a.cu[0] = 0;
-    if (tid == 0) *t.n_free = RESERVE ? n_free - base.a : n_free + base.a;
+    if (tid == 0) *t.n_free = RESERVE ? n_free - base.a : n_free + gone;
 }
 
 // The slots of many tokens, behind the tables kernel and over the whole chip: token x belongs to the request whose cu range holds it, and its

@@ -154,7 +154,7 @@ class PagedKVCache:
         return out.split_with_sizes((n_tokens, n_tokens, n + 1, 2))
 
     def truncate(self, seqs: torch.Tensor, lens: torch.Tensor) -> torch.Tensor:
-        """Sequences are cut to `lens` tokens (0 releases them) -> status [2]."""
+        """Sequences are cut to `lens` tokens (0 releases them) -> status [2].  Table entries that are no page give nothing back."""
         n = seqs.shape[0]
         sp, lp = self._ints("seqs", seqs), self._ints("lens", lens, n)
         status = torch.empty(2, dtype=torch.int32, device=self.device)

@@ -366,7 +366,8 @@ enum { AHA_PAGED_NO_PAGES = 1,     /* the free list is too short                
 int aha_paged_reserve(aha_paged* p, const int32_t* seqs, const int32_t* counts, int n, int32_t* slots, int32_t* positions, int n_tokens,
                       int32_t* cu_tokens, int32_t* status, aha_hip_stream st);
 /* Sequence seqs[i] is cut to new_lens[i] <= its length (0: it is released); its pages behind the last needed one return to the free list and
- * their table entries become -1.  The exact inverse of a reserve of the same sequences in the same order. */
+ * their table entries become -1.  Entries that are no page (dropped by the caller) give nothing back.  The exact inverse of a reserve of the
+ * same sequences in the same order. */
 int aha_paged_truncate(aha_paged* p, const int32_t* seqs, const int32_t* new_lens, int n, int32_t* status, aha_hip_stream st);
 /* One layer's new tokens: q [n_tokens][heads][head_dim] and k are rotated by the row positions[t] (clamped to 0 .. n_pos-1) of cos / sin (bf16
  * [n_pos][head_dim], the table of aha_ctx_set_rope_table; null: no rotation), q to q_out (may be q), k and v to the pages of their slots; a
