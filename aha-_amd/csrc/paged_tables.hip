@@ -11,7 +11,7 @@
 // sequence -> length -> sum -> free entry -> store, each link a trip to the L2 or memory.  All requests are looked at before anything is
 // written, so a call that cannot be done (status) changes nothing.  Pages and tokens are dealt out flat, a thread finds the request of its
 // page or token by bisection of the sums in LDS: a request of two thousand tokens does not keep one thread busy.  16 requests of a token: reserve
-// 4.2 us, truncate 3.0; 256 of some 250 tokens (64,700): 7.0 and 4.0 for the slots, truncate 5.9.
+// 4.2 us, truncate 3.7; 256 of some 250 tokens (64,700): 7.0 and 4.0 for the slots, truncate 6.7.
 #include "paged.h"
 
 struct Scan2 { int a, b; };
@@ -48,6 +48,7 @@ static __device__ __forceinline__ int bisect(const int* end, int n, int x) {
 }
 
 #define PT_THREADS 1024
+#define PT_KEEP 2
 struct Request { int seq, len, count, had, need, err; };     // had: pages it keeps; need: pages it takes (gives back)
 
 // What request i asks for; an entry with a negative sequence is padding and asks for nothing.
@@ -116,6 +117,12 @@ __global__ __launch_bounds__(PT_THREADS) void paged_tables_kernel(PagedReserveAr
     unsigned long long missing = 0;
     int gone = 0;                                              // truncate: pages that go back
     Scan2 all = {0, 0};
+    auto is_page = [&](int page) { return (unsigned)page < (unsigned)t.n_pages; };
+    auto entry = [&](int p, int m) {                           // of a chunk of requests, whose sums are in LDS: the table's entry of its p-th page
+        const int i = bisect(pend, m, p);
+        return t.table + (long)rseq[i] * t.max_blocks + rhad[i] + p - (i ? pend[i - 1] : 0);
+    };
+    int *kept[PT_KEEP], page_of[PT_KEEP];                      // truncate of at most NT requests: a thread's first entries
     if (err) {                                                 // the sums of requests that are none say nothing
     } else if (RESERVE) {
         if (pages > (unsigned long long)n_free) { err |= PAGED_NO_PAGES; missing = pages - n_free; }
@@ -123,19 +130,22 @@ __global__ __launch_bounds__(PT_THREADS) void paged_tables_kernel(PagedReserveAr
     } else if (pages > 0x7fffffffull - 4096) err |= PAGED_BAD_SEQ;          // (more than the sums below hold: no table has as many)
     else {
         // only entries that are pages go back: how many are there?
-        int good = 0;
+        int good = 0;                                          // of the wave, in its first lane (whose p is the least)
         for (int i0 = 0; i0 < a.n; i0 += NT) {
             const Request r = i0 ? look<RESERVE>(a, i0 + tid) : r0;
             pend[tid] = block_scan({r.need, 0}, wsum, &all).a; rseq[tid] = r.seq; rhad[tid] = r.had;
             __syncthreads();
             const int m = min(NT, a.n - i0);
-            for (int p = tid; p < all.a; p += NT) {
-                const int i = bisect(pend, m, p);
-                good += (unsigned)t.table[(long)rseq[i] * t.max_blocks + rhad[i] + p - (i ? pend[i - 1] : 0)] < (unsigned)t.n_pages;
-            }
+#pragma unroll
+            for (int k = 0; k < PT_KEEP; ++k) kept[k] = tid + k * NT < all.a ? entry(tid + k * NT, m) : nullptr;
+#pragma unroll
+            for (int k = 0; k < PT_KEEP; ++k) page_of[k] = kept[k] ? *kept[k] : -1;
+#pragma unroll
+            for (int k = 0; k < PT_KEEP; ++k) good += __popcll(__ballot(is_page(page_of[k])));
+            for (int p = tid + PT_KEEP * NT; p < all.a; p += NT) good += __popcll(__ballot(is_page(*entry(p, m))));
             __syncthreads();
         }
-        if (good) atomicAdd(&good_s, good);
+        if ((tid & 63) == 0) atomicAdd(&good_s, good);
         __syncthreads();
         gone = good_s;
         if ((long)gone + n_free > t.n_pages) err |= PAGED_BAD_SEQ;       // more pages than the pool has: the tables are not its own
@@ -167,26 +177,27 @@ __global__ __launch_bounds__(PT_THREADS) void paged_tables_kernel(PagedReserveAr
             __syncthreads();
         }
         const int m = min(NT, a.n - i0);
-        const bool whole = (unsigned long long)gone == pages;  // every entry is a page: the p-th entry is the p-th page
-        for (int p0 = 0; p0 < all.a; p0 += NT) {
-            const int p = p0 + tid;
-            int* e = nullptr;
-            if (p < all.a) {
-                const int i = bisect(pend, m, p);
-                e = t.table + (long)rseq[i] * t.max_blocks + rhad[i] + p - (i ? pend[i - 1] : 0);
-            }
-            if (RESERVE) {
-                if (e) *e = t.free_pages[n_free - 1 - (base.a + p)];
-            } else {
-                const int page = e ? *e : -1, good = (unsigned)page < (unsigned)t.n_pages;
-                int at = base.a + p;
-                if (!whole) {
+        if (RESERVE) {
+            for (int p = tid; p < all.a; p += NT) *entry(p, m) = t.free_pages[n_free - 1 - (base.a + p)];
+        } else {
+            auto give = [&](int p, int* e, int page) {         // (every thread calls it)
+                int at = base.a + p;                           // every entry is a page: the p-th entry is the p-th page
+                if ((unsigned long long)gone != pages) {
                     Scan2 here;
-                    at = back + block_scan({good, 0}, wsum, &here).a - good;
+                    at = back + block_scan({is_page(page), 0}, wsum, &here).a - is_page(page);
                     back += here.a;
                 }
-                if (good) t.free_pages[n_free + gone - 1 - at] = page;
+                if (is_page(page)) t.free_pages[n_free + gone - 1 - at] = page;
                 if (e) *e = -1;
+            };
+            int p0 = 0;
+            if (a.n <= NT)
+#pragma unroll
+                for (int k = 0; k < PT_KEEP; ++k, p0 += NT)
+                    if (p0 < all.a) give(p0 + tid, kept[k], page_of[k]);
+            for (; p0 < all.a; p0 += NT) {
+                int* e = p0 + tid < all.a ? entry(p0 + tid, m) : nullptr;
+                give(p0 + tid, e, e ? *e : -1);
             }
         }
         if (RESERVE && map_tokens)
