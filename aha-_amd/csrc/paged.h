@@ -9,7 +9,7 @@
 
 enum { PAGED_BF16 = 0, PAGED_E4M3 = 1 };
 // what reserve / truncate put in status[0] (a sum of these); with any of them set nothing was changed
-enum { PAGED_NO_PAGES = 1, PAGED_MANY_TOKENS = 2, PAGED_BAD_SEQ = 4, PAGED_TWICE = 8, PAGED_TOO_LONG = 16, PAGED_BAD_COUNT = 32 };
+enum { PAGED_NO_PAGES = 1, PAGED_MANY_TOKENS = 2, PAGED_BAD_SEQ = 4, PAGED_TWICE = 8, PAGED_TOO_LONG = 16, PAGED_BAD_COUNT = 32, PAGED_BAD_PAGE = 64 };
 #define PAGED_MAX_SEQS 65536                     // sequences of a pool: one bit each in LDS finds a sequence that is listed twice
 
 struct PagedTables {

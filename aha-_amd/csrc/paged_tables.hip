@@ -11,7 +11,7 @@
 // sequence -> length -> sum -> free entry -> store, each link a trip to the L2 or memory.  All requests are looked at before anything is
 // written, so a call that cannot be done (status) changes nothing.  Pages and tokens are dealt out flat, a thread finds the request of its
 // page or token by bisection of the sums in LDS: a request of two thousand tokens does not keep one thread busy.  16 requests of a token: reserve
-// 4.2 us, truncate 3.7; 256 of some 250 tokens (64,700): 7.0 and 4.0 for the slots, truncate 6.7.
+// 4.7 us, truncate 3.7; 256 of some 250 tokens (64,700): 7.7 and 4.0 for the slots, truncate 6.7.
 #include "paged.h"
 
 struct Scan2 { int a, b; };
@@ -49,12 +49,12 @@ static __device__ __forceinline__ int bisect(const int* end, int n, int x) {
 
 #define PT_THREADS 1024
 #define PT_KEEP 2
-struct Request { int seq, len, count, had, need, err; };     // had: pages it keeps; need: pages it takes (gives back)
+struct Request { int seq, len, count, had, need, last, err; };     // had: pages it keeps; need: pages it takes (gives back); last: its page that is filled in part
 
 // What request i asks for; an entry with a negative sequence is padding and asks for nothing.
 template <bool RESERVE>
 static __device__ __forceinline__ Request look(const PagedReserveArgs& a, int i) {
-    Request r = {-1, 0, 0, 0, 0, 0};
+    Request r = {-1, 0, 0, 0, 0, -1, 0};
     if (i >= a.n) return r;
     r.seq = a.seqs[i];
     const int c = a.counts[i];
@@ -71,6 +71,10 @@ static __device__ __forceinline__ Request look(const PagedReserveArgs& a, int i)
         r.count = c;
         r.had = (int)(((long)r.len + P1) >> lps);
         r.need = (int)(((long)r.len + c + P1) >> lps) - r.had;
+        if (c && (r.len & P1)) {                               // new tokens go to a page that it has
+            r.last = a.t.table[(long)r.seq * a.t.max_blocks + r.had - 1];
+            if ((unsigned)r.last >= (unsigned)a.t.n_pages) r.err = PAGED_BAD_PAGE;
+        }
     } else {
         if (c < 0 || c > r.len) { r.err = PAGED_BAD_COUNT; return r; }
         r.count = c;
@@ -84,17 +88,20 @@ template <bool RESERVE>
 __global__ __launch_bounds__(PT_THREADS) void paged_tables_kernel(PagedReserveArgs a, int map_tokens) {
     __shared__ unsigned seen[PAGED_MAX_SEQS / 32];
     __shared__ Scan2 wsum[PT_THREADS / 64];
-    __shared__ int pend[PT_THREADS], tend[PT_THREADS], rseq[PT_THREADS], rhad[PT_THREADS], rlen[PT_THREADS];
-    __shared__ int err_s, good_s;
+    __shared__ int pend[PT_THREADS], tend[PT_THREADS], rseq[PT_THREADS], rhad[PT_THREADS], rlen[PT_THREADS], rlast[PT_THREADS];
+    __shared__ int err_s, good_s, bad_at;
     __shared__ unsigned long long pages_s, tokens_s;
     const int tid = threadIdx.x, NT = blockDim.x;
     const PagedTables& t = a.t;
     const int words = (t.max_seqs + 31) >> 5;
     for (int i = tid; i < words; i += NT) seen[i] = 0;
-    if (tid == 0) { err_s = 0; good_s = 0; pages_s = 0; tokens_s = 0; }
+    if (tid == 0) { err_s = 0; good_s = 0; bad_at = 0x7fffffff; pages_s = 0; tokens_s = 0; }
     const int n_free = min(max(*t.n_free, 0), t.n_pages);
+    // the list's last entries, while the requests are looked at; an entry that is no page must not be handed out
+    const int e0 = RESERVE && tid < n_free ? t.free_pages[n_free - 1 - tid] : 0;
     Request r0 = look<RESERVE>(a, tid);                        // kept: with at most NT requests nothing is read twice
     __syncthreads();
+    if ((unsigned)e0 >= (unsigned)t.n_pages) atomicMin(&bad_at, tid);
 
     // ---- look at every request
     int err = 0;
@@ -127,6 +134,12 @@ __global__ __launch_bounds__(PT_THREADS) void paged_tables_kernel(PagedReserveAr
     } else if (RESERVE) {
         if (pages > (unsigned long long)n_free) { err |= PAGED_NO_PAGES; missing = pages - n_free; }
         if (tokens > (unsigned long long)a.n_tokens) err |= PAGED_MANY_TOKENS;
+        if (!err && pages > (unsigned long long)NT) {          // (uniform)
+            for (int p = tid + NT; p < (int)pages; p += NT)
+                if ((unsigned)t.free_pages[n_free - 1 - p] >= (unsigned)t.n_pages) atomicMin(&bad_at, p);
+            __syncthreads();
+        }
+        if (!err && (unsigned long long)bad_at < pages) err |= PAGED_BAD_PAGE;
     } else if (pages > 0x7fffffffull - 4096) err |= PAGED_BAD_SEQ;          // (more than the sums below hold: no table has as many)
     else {
         // only entries that are pages go back: how many are there?
@@ -169,7 +182,7 @@ __global__ __launch_bounds__(PT_THREADS) void paged_tables_kernel(PagedReserveAr
         const Request r = i0 ? look<RESERVE>(a, i0 + tid) : r0;
         if (RESERVE || a.n > NT) {                             // (else the count has left the sums as they are needed)
             const Scan2 in = block_scan({r.need, RESERVE ? r.count : 0}, wsum, &all);
-            pend[tid] = in.a; tend[tid] = in.b; rseq[tid] = r.seq; rhad[tid] = r.had; rlen[tid] = r.len;
+            pend[tid] = in.a; tend[tid] = in.b; rseq[tid] = r.seq; rhad[tid] = r.had; rlen[tid] = r.len; rlast[tid] = r.last;
             if (RESERVE && i0 + tid < a.n) {
                 a.cu[i0 + tid + 1] = base.b + in.b;
                 if (i0 + tid == 0) a.cu[0] = 0;
@@ -204,10 +217,9 @@ __global__ __launch_bounds__(PT_THREADS) void paged_tables_kernel(PagedReserveAr
             for (int x = tid; x < all.b; x += NT) {
                 const int i = bisect(tend, m, x), off = x - (i ? tend[i - 1] : 0);
                 const int pos = rlen[i] + off, blk = pos >> t.lps;
-                const int page = blk < rhad[i] ? t.table[(long)rseq[i] * t.max_blocks + blk]
-                                               : t.free_pages[n_free - 1 - (base.a + (i ? pend[i - 1] : 0) + blk - rhad[i])];
+                const int page = blk < rhad[i] ? rlast[i] : t.free_pages[n_free - 1 - (base.a + (i ? pend[i - 1] : 0) + blk - rhad[i])];
                 a.positions[base.b + x] = pos;
-                a.slots[base.b + x] = (unsigned)page < (unsigned)t.n_pages ? (page << t.lps) + (pos & ((1 << t.lps) - 1)) : -1;
+                a.slots[base.b + x] = (page << t.lps) + (pos & ((1 << t.lps) - 1));
             }
         if (r.seq >= 0) t.lens[r.seq] = RESERVE ? r.len + r.count : r.count;
         base.a += all.a; base.b += all.b;

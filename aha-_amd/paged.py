@@ -23,7 +23,7 @@ from . import lib as _l
 from .runtime import AhaError
 
 _ERRORS = ((1, "the free list is too short"), (2, "more new tokens than n_tokens"), (4, "a sequence out of range or a corrupt length"),
-           (8, "a sequence is listed twice"), (16, "a sequence outgrows its block table"), (32, "a negative count or a length out of range"))
+           (8, "a sequence is listed twice"), (16, "a sequence outgrows its block table"), (32, "a negative count or a length out of range"), (64, "a new token's page, from the free list or the block table, is none"))
 _TYPES = {torch.bfloat16: _l.KV_BF16, torch.float8_e4m3fn: _l.KV_E4M3}
 
 

@@ -362,7 +362,8 @@ enum { AHA_PAGED_NO_PAGES = 1,     /* the free list is too short                
        AHA_PAGED_BAD_SEQ = 4,      /* a sequence >= max_seqs, or a corrupt length        */
        AHA_PAGED_TWICE = 8,        /* a sequence is listed twice                         */
        AHA_PAGED_TOO_LONG = 16,    /* a sequence would outgrow max_blocks pages          */
-       AHA_PAGED_BAD_COUNT = 32 }; /* a negative count; truncate: a length out of 0..len */
+       AHA_PAGED_BAD_COUNT = 32,   /* a negative count; truncate: a length out of 0..len */
+       AHA_PAGED_BAD_PAGE = 64 };  /* new tokens would go to an entry, of the free list or of a sequence's table, that is no page */
 int aha_paged_reserve(aha_paged* p, const int32_t* seqs, const int32_t* counts, int n, int32_t* slots, int32_t* positions, int n_tokens,
                       int32_t* cu_tokens, int32_t* status, aha_hip_stream st);
 /* Sequence seqs[i] is cut to new_lens[i] <= its length (0: it is released); its pages behind the last needed one return to the free list and
