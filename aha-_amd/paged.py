@@ -221,10 +221,17 @@ class PagedKVCache:
 
     # -- a look at a sequence -----------------------------------------------------------------------------------------------
     def export_kv(self, layer: int, seq: int, want_v: bool = False) -> torch.Tensor:
-        """The keys (or values) of a sequence, [kv_heads, length, head_dim], scaled back to fp32 where the pool is e4m3.  A host round trip."""
+        """The keys (or values) of a sequence, [kv_heads, length, head_dim], scaled back to fp32 where the pool is e4m3; zeros where a table entry
+        is no page, whose keys attention hides.  A host round trip."""
+        if not (0 <= layer < self.layers and 0 <= seq < self.max_seqs):
+            raise ValueError(f"layer {layer} of {self.layers} or sequence {seq} of {self.max_seqs} is out of range")
         n = int(self.lens[seq])
+        if not 0 <= n <= self.max_blocks * self.page_size:
+            raise AhaError(f"paged cache: sequence {seq} has a corrupt length, {n}")
         pages = self.block_table[seq, :-(-n // self.page_size)].long()
-        x = (self.v_pages if want_v else self.k_pages)[layer].view(torch.uint8)[pages].view(self.dtype)
+        raw = (self.v_pages if want_v else self.k_pages)[layer].view(torch.uint8)[pages.clamp(0, self.n_pages - 1)]
+        raw[(pages < 0) | (pages >= self.n_pages)] = 0
+        x = raw.view(self.dtype)
         x = x.transpose(0, 1).reshape(self.kv_heads, -1, self.head_dim)[:, :n]
         if self.dtype == torch.float8_e4m3fn:
             s = self.v_scale if want_v else self.k_scale
