@@ -25,6 +25,12 @@ from .runtime import AhaError
 _ERRORS = ((1, "the free list is too short"), (2, "more new tokens than n_tokens"), (4, "a sequence out of range or a corrupt length"),
            (8, "a sequence is listed twice"), (16, "a sequence outgrows its block table"), (32, "a negative count or a length out of range"), (64, "a new token's page, from the free list or the block table, is none"))
 _TYPES = {torch.bfloat16: _l.KV_BF16, torch.float8_e4m3fn: _l.KV_E4M3}
+_MAX = 0x7fffffff
+
+
+def _c_ints(*x):
+    """As the library's 32-bit arguments: what lies beyond them at their nearer end, where it means or is refused as the same (ctypes would cut the bits off)."""
+    return [max(-_MAX - 1, min(int(i), _MAX)) for i in x]
 
 
 class PagedKVCache:
@@ -50,6 +56,8 @@ class PagedKVCache:
         shape = (self.layers, self.n_pages, self.kv_heads, self.page_size, self.head_dim)
         if min(shape + (self.max_seqs, self.max_blocks)) < 1:
             raise ValueError("sizes must be positive")
+        if max(shape + (self.max_seqs, self.max_blocks)) > _MAX:
+            raise ValueError("sizes must be below 2^31")
         if free_pages is not None and n_free is None:
             raise ValueError("free_pages needs n_free")
         self.k_pages = self._own("k_pages", k_pages, shape, dtype)
@@ -71,7 +79,7 @@ class PagedKVCache:
                 self._own(name, t, (rows, self.head_dim), torch.bfloat16)
             if rows < 1:
                 raise ValueError("rope: cos and sin must be [positions, head_dim]")
-            self._rope = (self.cos.data_ptr(), self.sin.data_ptr(), rows)
+            self._rope = (self.cos.data_ptr(), self.sin.data_ptr(), min(rows, _MAX))
         d = _l.PagedDesc(k_pages=self.k_pages.data_ptr(), v_pages=self.v_pages.data_ptr(), block_table=self.block_table.data_ptr(),
                          lens=self.lens.data_ptr(), free_pages=self.free_pages.data_ptr(), n_free=self.n_free.data_ptr(),
                          k_scale=self.k_scale.data_ptr() if self.k_scale is not None else None,
@@ -145,12 +153,12 @@ class PagedKVCache:
     def reserve(self, seqs: torch.Tensor, counts: torch.Tensor, n_tokens: int):
         """Sequences grow by `counts` tokens, at most `n_tokens` in all -> (slots [n_tokens], positions [n_tokens], cu [n + 1], status [2])."""
         n = seqs.shape[0]
-        if n_tokens < 0:
-            raise ValueError("n_tokens must not be negative")
+        if not 0 <= n_tokens <= _MAX - 4096:
+            raise ValueError(f"n_tokens must be 0 .. {_MAX - 4096}")
         sp, cp = self._ints("seqs", seqs), self._ints("counts", counts, n)
         out = torch.empty(2 * n_tokens + n + 3, dtype=torch.int32, device=self.device)
         p = out.data_ptr()
-        self._chk(self.lib.aha_paged_reserve(self.handle, sp, cp, n, p, p + 4 * n_tokens, n_tokens, p + 8 * n_tokens, p + 8 * n_tokens + 4 * (n + 1), self._stream()))
+        self._chk(self.lib.aha_paged_reserve(self.handle, sp, cp, min(n, _MAX), p, p + 4 * n_tokens, n_tokens, p + 8 * n_tokens, p + 8 * n_tokens + 4 * (n + 1), self._stream()))
         return out.split_with_sizes((n_tokens, n_tokens, n + 1, 2))
 
     def truncate(self, seqs: torch.Tensor, lens: torch.Tensor) -> torch.Tensor:
@@ -158,7 +166,7 @@ class PagedKVCache:
         n = seqs.shape[0]
         sp, lp = self._ints("seqs", seqs), self._ints("lens", lens, n)
         status = torch.empty(2, dtype=torch.int32, device=self.device)
-        self._chk(self.lib.aha_paged_truncate(self.handle, sp, lp, n, status.data_ptr(), self._stream()))
+        self._chk(self.lib.aha_paged_truncate(self.handle, sp, lp, min(n, _MAX), status.data_ptr(), self._stream()))
         return status
 
     def append(self, layer: int, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, positions: Optional[torch.Tensor] = None,
@@ -186,6 +194,8 @@ class PagedKVCache:
                 if q_out.shape[0] != n:
                     raise ValueError("q_out needs as many tokens as q")
             qp, op = q.data_ptr(), q_out.data_ptr()
+        if (layer | n | heads) >> 31:
+            layer, n, heads = _c_ints(layer, n, heads)
         self._chk(self.lib.aha_paged_append(self.handle, layer, qp, ldq, heads, op, ldo, k.data_ptr(), ldk, v.data_ptr(), ldv, sp, pp, n, cos, sin, rows, self._stream()))
         return q_out
 
@@ -204,8 +214,10 @@ class PagedKVCache:
             out, _, ldo = self._rows("out", out, heads, out=True)
             if out.shape[0] != N:
                 raise ValueError("out needs as many tokens as q")
-        if window > 0x7fffffff:                                    # (more than a sequence can hold: all keys)
+        if window > _MAX:                                          # (more than a sequence can hold: all keys)
             window = 0
+        if (layer | N | n | heads | max_q | max_len | window) >> 31:
+            layer, N, n, heads, max_q, max_len, window = _c_ints(layer, N, n, heads, max_q, max_len, window)
         key = (heads, N, n, max_q, max_len)
         need = self._workspace.get(key)
         if need is None:                                           # (a function of the sizes alone, asked for once)
