@@ -206,6 +206,13 @@ static __device__ __forceinline__ void no_keys(const PagedAttnArgs& a, int slot,
         ml[0] = -INFINITY; ml[1] = 0.f;
     }
 }
+// what turns a product of q and k into an exponent of 2.  Never zero (keys of a head with scale 0, or a product of scales below the least float): hidden
+// scores are -infinity before it is applied, and -infinity * 0 is no number; at the least normal number every visible score still is one of 0.
+template <bool E4M3>
+static __device__ __forceinline__ float log2_scale(const PagedAttnArgs& a, int hk) {
+    const float c = a.scale * (E4M3 && a.k_scale ? a.k_scale[hk] : 1.f) * 1.4426950408889634f;
+    return c == 0.f ? 1.17549435e-38f : c;
+}
 static __device__ __forceinline__ bool nonfinite(bf16x8 v) {
     const u32x4 u = __builtin_bit_cast(u32x4, v);
     bool bad = false;
@@ -263,7 +270,7 @@ __global__ __launch_bounds__(256) void paged_attn_rows_kernel(PagedAttnArgs a) {
     }
     const int pos_min = base_pos + quot(w.tile * TR, a.by_G), pos_max = base_pos + min(quot(w.tile * TR + TR - 1, a.by_G), w.T - 1);
     const bool one_pos = pos_min == pos_max;
-    const float c2 = a.scale * (E4M3 && a.k_scale ? a.k_scale[hk] : 1.f) * 1.4426950408889634f;
+    const float c2 = log2_scale<E4M3>(a, hk);
 
     f32x4 o[DT];
     float m_run = -INFINITY, l_run = 0.f;
@@ -530,7 +537,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
     // the positions of the workgroup's rows, and of the wave's
     const int pos_lo = base_pos + quot(w.tile * TR, a.by_G), pos_hi = base_pos + min(quot(w.tile * TR + TR - 1, a.by_G), w.T - 1);
     const int wpos_lo = base_pos + quot(min(row0, R - 1), a.by_G), wpos_hi = base_pos + quot(min(row0 + 16 * NT - 1, R - 1), a.by_G);
-    const float c2 = a.scale * (E4M3 && a.k_scale ? a.k_scale[hk] : 1.f) * 1.4426950408889634f;
+    const float c2 = log2_scale<E4M3>(a, hk);
 
     f32x4 o[NT][DT], lacc[NT];
     float m_run[NT];

@@ -36,7 +36,7 @@ def _c_ints(*x):
 class PagedKVCache:
     """One pool.  `rope`: (cos, sin), bf16 [positions, head_dim], what `append` rotates with
     (positions behind its last as the last); without it keys and queries come rotated.
-    `k_scale` / `v_scale`: fp32 [layers, kv_heads] of an e4m3 pool (default 1).  The tensors (`k_pages`, `v_pages`: [layers, n_pages, kv_heads,
+    `k_scale` / `v_scale`: fp32 [layers, kv_heads] of an e4m3 pool (default 1), finite and not negative (0: that head's values are 0).  The tensors (`k_pages`, `v_pages`: [layers, n_pages, kv_heads,
     page_size, head_dim]; `block_table` [max_seqs, max_blocks], `lens` [max_seqs], `free_pages` [n_pages], `n_free` [1], all int32) are made
     here unless given, and are the caller's to look at; pages may hold anything."""
 

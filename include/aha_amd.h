@@ -344,7 +344,7 @@ typedef struct aha_paged_desc {
     int32_t* block_table;                     /* [max_seqs][max_blocks]: page of each run of page_size tokens; entries behind the last are ignored */
     int32_t* lens;                            /* [max_seqs]: tokens of each sequence */
     int32_t *free_pages, *n_free;             /* [n_pages], [1]: the free list is free_pages[0 .. *n_free) and is taken from its end */
-    const float *k_scale, *v_scale;           /* [layers][kv_heads], E4M3 only; null = 1 */
+    const float *k_scale, *v_scale;           /* [layers][kv_heads], E4M3 only; null = 1.  Finite and not negative; 0: the head's values are 0 */
     int32_t layers, n_pages, page_size;       /* page_size: a power of two, 16 .. 1024 */
     int32_t kv_heads, head_dim;               /* head_dim: a multiple of 16, at most 128 */
     int32_t kv_type, max_seqs, max_blocks;    /* max_seqs <= 65536 */

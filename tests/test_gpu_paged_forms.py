@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import aha_amd  # noqa: F401
-from test_gpu_paged import check_attention, filled, gen, ints, randn
+from test_gpu_paged import DEV, check_attention, filled, gen, ints, pool, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -12,3 +12,34 @@ pytestmark = pytest.mark.gpu
 def test_hints_of_any_width(hints):
     c = filled([700, 90], 16, 28, 4, 128, "bf16", 17)
     check_attention(c, randn(gen(18), 132, 28, 128).bfloat16(), ints([0, 1]), ints([0, 131, 132]), **hints)
+
+
+@pytest.mark.parametrize("T", [1, 3, 40, 150])
+@pytest.mark.parametrize("window", [0, 70])
+def test_a_head_whose_scale_is_zero(T, window):
+    """Its keys are all zero, so every visible key weighs the same; hidden ones still nothing.  Another head's values are zero."""
+    c = filled([700, 90, T], 16, 12, 4, 128, "e4m3", 41 + T)
+    c.k_scale[0, 1], c.v_scale[0, 2] = 0.0, 0.0
+    q = (randn(gen(42), 3 * T, 12, 128) * 1.5).bfloat16()
+    got = check_attention(c, q, ints([0, 1, 2]), ints([0, T, 2 * T, 3 * T]), window=window, max_q=T)
+    assert not bool(got.view(-1, 4, 3, 128)[:, 2].any())
+
+
+@pytest.mark.parametrize("T", [1, 40])
+@pytest.mark.parametrize("scale", [1e-38, 2e-45])
+def test_scales_whose_product_is_below_the_least_float(T, scale):
+    c = filled([700, 90], 16, 8, 2, 64, "e4m3", 43)
+    c.k_scale.fill_(1e-12)
+    check_attention(c, randn(gen(44), 2 * T, 8, 64).bfloat16(), ints([0, 1]), ints([0, T, 2 * T]), scale=scale, max_q=T)
+
+
+def test_append_with_a_scale_of_zero_stores_zero():
+    c = pool(1, 16, 1, 1, 2, 16, dtype=torch.float8_e4m3fn, k_scale=torch.tensor([[0.0, 0.5]], device=DEV), v_scale=torch.tensor([[0.5, 0.0]], device=DEV))
+    x = torch.tensor([[0.0, -0.0, 3.0, -1e4, float("inf"), -float("inf"), float("nan"), 2 ** -20] * 4], device=DEV).bfloat16()
+    c.append(0, None, x, x, ints([0]))
+    for pages, zero in ((c.k_pages, 0), (c.v_pages, 1)):
+        got = pages[0, 0, :, 0].float()
+        nan = torch.isnan(x.view(2, 16)[0])
+        assert torch.equal(torch.isnan(got[zero]), nan) and not bool(got[zero][~nan].any())
+        other = (x.view(2, 16)[1 - zero].float() / 0.5).clamp(-448, 448)
+        assert torch.equal(got[1 - zero][~nan], other[~nan].to(torch.float8_e4m3fn).float())
