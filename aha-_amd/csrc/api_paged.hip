@@ -12,6 +12,7 @@ struct aha_paged {
     aha_paged_desc d;
     int device, lps;
     std::atomic<int> n_cus;                      // asked for once, by the first attention call
+    std::atomic<int> precise;
 };
 
 static thread_local char g_paged_err[256];
@@ -71,9 +72,14 @@ extern "C" int aha_paged_create(const aha_paged_desc* d, int device, aha_paged**
     if ((int64_t)d->max_blocks * d->page_size > 0x7fffffff - 4096) return refuse(E_RANGE, "sequences of more than 2^31 - 4097 tokens");
     aha_paged* p = new (std::nothrow) aha_paged();
     if (!p) return refuse(E_NOMEM, "out of memory");
-    p->d = *d; p->device = device; p->lps = 0; p->n_cus = 0;
+    p->d = *d; p->device = device; p->lps = 0; p->n_cus = 0; p->precise = 0;
     while ((1 << p->lps) < d->page_size) ++p->lps;
     *out = p;
+    return 0;
+}
+extern "C" int aha_paged_set_precise(aha_paged* p, int on) {
+    if (!p) return refuse(E_INVAL, "null handle");
+    p->precise = on != 0;
     return 0;
 }
 extern "C" void aha_paged_destroy(aha_paged* p) { delete p; }
@@ -193,7 +199,7 @@ extern "C" int aha_paged_attention(aha_paged* p, int layer, const void* q, int64
     a.k_scale = d.k_scale ? d.k_scale + (size_t)layer * d.kv_heads : nullptr;
     a.v_scale = d.v_scale ? d.v_scale + (size_t)layer * d.kv_heads : nullptr;
     a.table = d.block_table; a.lens = d.lens; a.seqs = seqs; a.cu = cu_tokens;
-    a.window = window; a.scale = scale;
+    a.window = window; a.scale = scale; a.precise = p->precise;
     a.most_keys = window && window < 0x7fffffff - a.tile_rows - 65 ? window + a.tile_rows / a.G + 65 : 0x7fffffff;
     a.part_o = (float*)workspace;
     a.part_ml = need ? a.part_o + paged_partial_floats(&a) : nullptr;

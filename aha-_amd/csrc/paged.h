@@ -50,6 +50,7 @@ struct PagedAttnArgs {
     int most_keys;                               // that a tile's rows see between them
     PagedDiv by_G, by_kv_heads, by_heads;
     int grid_items, tile_rows;                   // workgroups a key-value head; rows of a tile
+    int precise;                                 // tiles of many rows: P as two bf16 halves
 };
 
 hipError_t paged_reserve(const PagedReserveArgs* a, hipStream_t st);
@@ -59,3 +60,4 @@ hipError_t paged_append(const PagedAppendArgs* a, hipStream_t st);
 size_t paged_attention_plan(PagedAttnArgs* a, int n_cus, int max_q, int max_len);
 size_t paged_partial_floats(const PagedAttnArgs* a);          // floats of part_o; part_ml and info lie behind them
 hipError_t paged_attention(const PagedAttnArgs* a, int e4m3, hipStream_t st);
+void paged_tiles_halves(const PagedAttnArgs* a, int e4m3, hipStream_t st);      // its launch of tiles, with P as two halves

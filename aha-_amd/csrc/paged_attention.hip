@@ -228,6 +228,7 @@ static __device__ __forceinline__ bf16x8 e4m3x8(unsigned lo, unsigned hi) {     
     return r;
 }
 
+#ifndef PAGED_HALVES
 // ---------------------------------------------------------------------------------------------
 // Few rows (one token: the G rows of a key-value head): bound by the bytes of K and V.  A workgroup's four waves take blocks of 32 keys in turn,
 // each with a softmax of its own and no barrier in the loop, and are merged at the end.  The matrix cores have time to spare, so P goes into
@@ -475,13 +476,15 @@ __global__ __launch_bounds__(256) void paged_attn_rows_kernel(PagedAttnArgs a) {
     }
 }
 
+#endif
 // ---------------------------------------------------------------------------------------------
 // Many rows (frames, prompts): bound by the matrix cores and the exponentials.  A workgroup's four waves have 16 NT rows each and share blocks of
 // 64 keys, K and V double-buffered in LDS: the next block is under way while this one is computed, with one barrier a block.  bf16 pages go
 // straight to LDS (buffer_load ... lds, 1 KiB of contiguous rows an instruction), e4m3 through registers, where they become bf16.  In LDS a row's
 // 16-byte chunks are permuted by its number: sixteen rows read at one column, or eight rows at two, touch every bank once.
-// P is rounded to bf16 (half a step, 2^-8 of p, as the output itself is); the sum of the row is taken from the rounded values, by the matrix cores
-// (a product with ones), so that numerator and denominator round alike.  The running maximum moves only when a score exceeds it by 2^8: until
+// P is rounded to bf16 (half a step, 2^-8 of p, as the output itself is) unless the caller asks for two halves (HALVES: 2^-17); the sum of the row is
+// taken from the rounded values, by the matrix cores (a product with ones), so that numerator and denominator round alike.  One half / two, us: 8,192
+// tokens over as many keys 487 / 703, 8 x 36 over 12,000 78 / 101, 16 x 5 over 5,000 39.8 / 40.4, x 7 in e4m3 30.5 / 34.8.  The running maximum moves only when a score exceeds it by 2^8: until
 // then the exponentials stay below 2^8 and neither the sum nor the output is rescaled.  28 / 4 heads of 128: 8,192 tokens over as many keys 481 us,
 // 1,000 TFLOP/s of the pairs a row sees (a large library product: 1,430), 8 / 2 heads of 64 562; 4 x 2,048 over 8,192 keys 848 us,
 // of which 800 stay without the exponentials, 751 without staging, 738 without the second product: none of them alone bounds it.  8 x 36 tokens
@@ -499,7 +502,7 @@ static __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t from, 
 #endif
 }
 
-template <int D, bool E4M3, int NT>
+template <int D, bool E4M3, int NT, bool HALVES>
 __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a) {
     constexpr int KSQ = D / 32, DT = D / 16, TR = 64 * NT, BLK = 64 * D;
     using LD = TileLds<D>;
@@ -687,7 +690,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
                         }
                 }
             }
-            bf16x8 pb[NT][2];
+            bf16x8 pb[NT][2], pr[HALVES ? NT : 1][2];           // P, and what its rounding left
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 // exponentials against the running reference; only where one of them exceeds 2^8, or a row has no reference yet, is the
@@ -725,9 +728,16 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
 #pragma unroll
                 for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) pb[nt][kt >> 1][(kt & 1) * 4 + e] = f2bf(p[kt][e]);
+                    for (int e = 0; e < 4; ++e) {
+                        const bf16 hi = f2bf(p[kt][e]);
+                        pb[nt][kt >> 1][(kt & 1) * 4 + e] = hi;
+                        if constexpr (HALVES) pr[nt][kt >> 1][(kt & 1) * 4 + e] = f2bf(p[kt][e] - bf2f(hi));
+                    }
 #pragma unroll
-                for (int kp_ = 0; kp_ < 2; ++kp_) lacc[nt] = mfma16(ones, pb[nt][kp_], lacc[nt]);
+                for (int kp_ = 0; kp_ < 2; ++kp_) {
+                    lacc[nt] = mfma16(ones, pb[nt][kp_], lacc[nt]);
+                    if constexpr (HALVES) lacc[nt] = mfma16(ones, pr[nt][kp_], lacc[nt]);
+                }
             }
             // O^T += V^T P^T: slot (q4, e) of a pair of key tiles is key 4 q4 + e of the first, of the second from e = 4
             const int vrow = 4 * q4 + (r16 >> 2), vch = (r16 & 3) >> 1, vin = 4 * (r16 & 1);
@@ -745,12 +755,15 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
                         const bf16x8 vf = v_frag(dt, kp_);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) o[nt][dt] = mfma16(vf, pb[nt][kp_], o[nt][dt]);
+                        if constexpr (HALVES)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) o[nt][dt] = mfma16(vf, pr[nt][kp_], o[nt][dt]);
                     }
                 if constexpr (!E4M3) {                      // (the registers of an e4m3 block under way leave no room)
                     __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);    // V fragments two channel tiles ahead
 #pragma unroll
                     for (int dt = 0; dt < DT; ++dt) {
-                        __builtin_amdgcn_sched_group_barrier(0x8, 2 * NT, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x8, (HALVES ? 4 : 2) * NT, 0);
                         if (dt + 2 < DT) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
                     }
                 }
@@ -771,7 +784,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
                             }
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt) {
-                                const f32x4 x = mfma16(vf, pb[nt][kp_], o[nt][dt]);
+                                f32x4 x = mfma16(vf, pb[nt][kp_], o[nt][dt]);
+                                if constexpr (HALVES) x = mfma16(vf, pr[nt][kp_], x);
                                 o[nt][dt] = pos[nt] == p ? x : o[nt][dt];
                             }
                         }
@@ -805,6 +819,21 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
     }
 }
 
+template <int D, bool E4M3, int TR, bool HALVES>
+static void launch_tiles(const PagedAttnArgs* a, hipStream_t st) {
+    paged_attn_tile_kernel<D, E4M3, TR / 64, HALVES><<<a->grid_items * a->kv_heads, 256, 4 * 64 * D * sizeof(bf16), st>>>(*a);
+}
+#ifdef PAGED_HALVES                                             // (a source of its own, built beside this one: paged_attention_halves.hip)
+template <int D, bool E4M3>
+static void launch_halves(const PagedAttnArgs* a, hipStream_t st) {
+    if (a->tile_rows == 64) launch_tiles<D, E4M3, 64, true>(a, st);
+    else launch_tiles<D, E4M3, 128, true>(a, st);
+}
+void paged_tiles_halves(const PagedAttnArgs* a, int e4m3, hipStream_t st) {
+    if (a->hd <= 64) e4m3 ? launch_halves<64, true>(a, st) : launch_halves<64, false>(a, st);
+    else e4m3 ? launch_halves<128, true>(a, st) : launch_halves<128, false>(a, st);
+}
+#else
 // ---------------------------------------------------------------------------------------------
 // Joins the chunks of split rows: a wave for each token (of many tokens most have nothing to join), for each token and query head, or, where that
 // leaves the chip empty, four waves for each token and head, which share its chunks.  A lane knows one chunk's maximum and sum, so the weights of
@@ -946,9 +975,10 @@ size_t paged_attention_plan(PagedAttnArgs* a, int n_cus, int max_q, int max_len)
 
 template <int D, bool E4M3, int TR>
 static hipError_t launch(const PagedAttnArgs* a, hipStream_t st) {
-    const int grid = a->grid_items * a->kv_heads;
-    if constexpr (TR > 16) paged_attn_tile_kernel<D, E4M3, TR / 64><<<grid, 256, 4 * 64 * D * sizeof(bf16), st>>>(*a);
-    else paged_attn_rows_kernel<D, E4M3><<<grid, 256, 0, st>>>(*a);
+    if constexpr (TR > 16) {
+        if (a->precise) paged_tiles_halves(a, E4M3, st);
+        else launch_tiles<D, E4M3, TR, false>(a, st);
+    } else paged_attn_rows_kernel<D, E4M3><<<a->grid_items * a->kv_heads, 256, 0, st>>>(*a);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && a->cmax > 1) {
         // of many tokens a wave looks at all heads of one: mostly there is nothing to join (8,192 tokens: 5 us, with a wave a head 35 us); of few
@@ -969,3 +999,4 @@ hipError_t paged_attention(const PagedAttnArgs* a, int e4m3, hipStream_t st) {
     if (template_dim(a) == 64) return e4m3 ? launch<64, true>(a, st) : launch<64, false>(a, st);
     return e4m3 ? launch<128, true>(a, st) : launch<128, false>(a, st);
 }
+#endif

@@ -101,6 +101,7 @@ SYMBOLS = [
     ("aha_comm_last_error", C.c_char_p, []),
     ("aha_paged_create", _I, [C.POINTER(PagedDesc), _I, C.POINTER(_P)]),
     ("aha_paged_destroy", None, [_P]),
+    ("aha_paged_set_precise", _I, [_P, _I]),
     ("aha_paged_last_error", C.c_char_p, []),
     ("aha_paged_reserve", _I, [_P, _P, _P, _I, _P, _P, _I, _P, _P, _P]),
     ("aha_paged_truncate", _I, [_P, _P, _P, _I, _P, _P]),

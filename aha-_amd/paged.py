@@ -38,13 +38,15 @@ class PagedKVCache:
     (positions behind its last as the last); without it keys and queries come rotated.
     `k_scale` / `v_scale`: fp32 [layers, kv_heads] of an e4m3 pool (default 1), finite and not negative (0: that head's values are 0).  The tensors (`k_pages`, `v_pages`: [layers, n_pages, kv_heads,
     page_size, head_dim]; `block_table` [max_seqs, max_blocks], `lens` [max_seqs], `free_pages` [n_pages], `n_free` [1], all int32) are made
-    here unless given, and are the caller's to look at; pages may hold anything."""
+    here unless given, and are the caller's to look at; pages may hold anything.  `precise`: the attention of drafts, frames and prompts keeps its
+    probabilities to 2^-17 (a token's always are) instead of rounding them to bf16, as the ring caches' attention does; up to half as slow again."""
 
     def __init__(self, n_pages: int, page_size: int, kv_heads: int, head_dim: int, max_seqs: int, max_blocks: int, *, layers: int = 1,
                  dtype: torch.dtype = torch.bfloat16, device="cuda:0", rope: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
                  k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None, k_pages: Optional[torch.Tensor] = None,
                  v_pages: Optional[torch.Tensor] = None, block_table: Optional[torch.Tensor] = None, lens: Optional[torch.Tensor] = None,
-                 free_pages: Optional[torch.Tensor] = None, n_free: Optional[torch.Tensor] = None):
+                 free_pages: Optional[torch.Tensor] = None, n_free: Optional[torch.Tensor] = None,
+                 precise: bool = False):
         self.handle = None
         self.lib = _l.get()
         dev = torch.device(device)
@@ -89,6 +91,8 @@ class PagedKVCache:
         h = C.c_void_p()
         self._chk(self.lib.aha_paged_create(C.byref(d), self.device.index or 0, C.byref(h)))
         self.handle = h
+        if precise:
+            self._chk(self.lib.aha_paged_set_precise(h, 1))
         self._workspace = {}                                       # sizes of a call -> bytes of its workspace
 
     # -- plumbing -----------------------------------------------------------------------------------------------------------

@@ -182,7 +182,8 @@ class Runtime:
     def open_paged(self, n_pages: int, max_seqs: int, *, page_size: int = 64, max_blocks: Optional[int] = None,
                    dtype: torch.dtype = torch.bfloat16, **tensors):
         """A paged key-value cache (aha_amd.paged.PagedKVCache) for this model: its layers, key-value heads and RoPE table; max_blocks pages a
-        sequence (default: as many as the table has positions for; beyond them a token is rotated as the last).  `tensors`: scales or storage of the caller's."""
+        sequence (default: as many as the table has positions for; beyond them a token is rotated as the last).  `tensors`: scales or
+        storage of the caller's, `precise`."""
         from .paged import PagedKVCache
         d = self.desc
         return PagedKVCache(n_pages, page_size, d.kv_heads, d.head_dim, max_seqs, max_blocks or max(1, d.max_positions // page_size), layers=d.layers, dtype=dtype,

@@ -351,6 +351,10 @@ typedef struct aha_paged_desc {
 } aha_paged_desc;
 int aha_paged_create(const aha_paged_desc* desc, int device, aha_paged** out);
 void aha_paged_destroy(aha_paged* p);
+/* How exact the attention of many rows is (more than sixteen tokens x heads of a key-value head: drafts, frames, prompts).  Off, as a pool is made:
+ * the probabilities are rounded to bf16 for the second product, 2^-8 of each, as aha_attention_forward does.  On: they go in as two bf16 halves, 2^-17,
+ * as those of fewer rows always do; up to half as slow again.  Two handles over the same memory may differ. */
+int aha_paged_set_precise(aha_paged* p, int on);
 const char* aha_paged_last_error(void);
 /* Sequence seqs[i] grows by counts[i] tokens, i < n (a negative sequence is padding and its count ignored).  Pages are taken from the end of
  * the free list in the order of the requests.  Out: cu_tokens [n+1], the running sum of the counts; slots / positions [n_tokens], of the

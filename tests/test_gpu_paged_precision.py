@@ -53,3 +53,59 @@ def test_few_tokens_of_a_small_group(heads, kv_heads, dim, T, kind):
 def test_a_token_over_a_long_sequence(kind, L):
     c = filled([L, 40], 64, 28, 4, 128, kind, L)
     check_tight(c, randn(gen(3), 2, 28, 128).bfloat16(), ints([0, 1]), ints([0, 1, 2]), max_q=1, max_len=L)
+
+
+def precisely(c):
+    c._chk(c.lib.aha_paged_set_precise(c.handle, 1))
+    return c
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", LAYOUTS)
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_a_precise_pool_keeps_the_bound_with_many_rows(heads, kv_heads, dim, kind):
+    """Drafts, frames and prompts, cut and whole, in tiles of 64 and of 128 rows, with a window and without."""
+    lens = [150, 36, 700, 300, 5, 129, 3]
+    counts = [2, 36, 131, 0, 5, 49, 5]                                       # (the last has more tokens than keys)
+    c = precisely(filled(lens, 32, heads, kv_heads, dim, kind, dim))
+    cu = ints([0] + torch.tensor(counts).cumsum(0).tolist())
+    q = (randn(gen(2), sum(counts), heads, dim) * 1.5).bfloat16()
+    whole = check_tight(c, q, ints(range(7)), cu, max_q=131, max_len=256)
+    check_tight(c, q, ints(range(7)), cu)
+    check_tight(c, q, ints(range(7)), cu, window=40, max_q=131)
+    few = torch.cat([q[cu[i]:cu[i] + 5] for i in (1, 2, 4)])
+    check_tight(c, few, ints([1, 2, 4]), ints([0, 5, 10, 15]), max_q=5)
+    assert torch.equal(c.attention(0, q, ints(range(7)), cu, max_q=131, max_len=256), whole)
+
+
+@pytest.mark.parametrize("T,L,kind", [(5, 3000, "bf16"), (36, 2500, "bf16"), (36, 2500, "e4m3"), (300, 1500, "e4m3")])
+def test_a_precise_pool_over_long_sequences(T, L, kind):
+    c = precisely(filled([L, 40], 64, 28, 4, 128, kind, L))
+    n = T + 1
+    check_tight(c, randn(gen(3), n, 28, 128).bfloat16(), ints([0, 1]), ints([0, T, n]), max_q=T, max_len=L)
+
+
+@pytest.mark.parametrize("T,kind", [(6, "bf16"), (40, "bf16"), (140, "e4m3")])
+def test_a_value_that_is_not_finite_in_a_precise_pool(T, kind):
+    """Reaches the rows that see its key, no others."""
+    L = 200
+    c = precisely(filled([L], 16, 7, 1, 128, kind, 11))
+    raw = c.v_pages.view(torch.uint8 if kind == "e4m3" else torch.int16)
+    for j in (L - 2, L - T // 2 - 1):
+        raw[0, int(c.block_table[0, j // 16]), 0, j % 16, 3] = 0x7f if kind == "e4m3" else 0x7fc0
+    got = check_tight(c, randn(gen(7), T, 7, 128).bfloat16(), ints([0]), ints([0, T]), window=20, max_q=T)
+    assert bool(torch.isnan(got[-1, 0, 3])) and not bool(torch.isnan(got[0].float()).any())
+
+
+def test_the_choice_is_the_handles():
+    """Two handles over the same memory, one precise: each keeps its own, a token has the same bits in both, and it can be switched off again."""
+    from aha_amd.paged import PagedKVCache
+    a = filled([700, 300], 16, 28, 4, 128, "bf16", 5)
+    b = PagedKVCache(a.n_pages, 16, 4, 128, 2, a.max_blocks, device=DEV, k_pages=a.k_pages, v_pages=a.v_pages, block_table=a.block_table, lens=a.lens,
+                     free_pages=a.free_pages, n_free=a.n_free, precise=True)
+    seqs, cu, one = ints([0, 1]), ints([0, 40, 80]), ints([0, 1, 2])
+    q = randn(gen(9), 80, 28, 128).bfloat16()
+    rounded, exact = a.attention(0, q, seqs, cu, max_q=40), check_tight(b, q, seqs, cu, max_q=40)
+    assert not torch.equal(rounded, exact)
+    assert torch.equal(a.attention(0, q[:2], seqs, one, max_q=1), b.attention(0, q[:2], seqs, one, max_q=1))
+    b._chk(b.lib.aha_paged_set_precise(b.handle, 0))
+    assert torch.equal(b.attention(0, q, seqs, cu, max_q=40), rounded)

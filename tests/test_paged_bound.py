@@ -28,3 +28,8 @@ def test_one_rounding_of_p_breaks_the_bound_and_two_halves_keep_it(dim, keys):
         out, exact, mag, size = attend(q, k, v, halves)
         off = (out - exact).abs() - U * exact.abs() - tight(dim, size, keys) * mag
         assert (float(off.max()) <= 0) == kept, (halves, float(off.max()), int((off > 0).sum()))
+
+
+def test_no_handle_no_choice():
+    from aha_amd import lib
+    assert lib.get().aha_paged_set_precise(None, 1) == -22
