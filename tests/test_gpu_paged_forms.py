@@ -43,3 +43,42 @@ def test_append_with_a_scale_of_zero_stores_zero():
         assert torch.equal(torch.isnan(got[zero]), nan) and not bool(got[zero][~nan].any())
         other = (x.view(2, 16)[1 - zero].float() / 0.5).clamp(-448, 448)
         assert torch.equal(got[1 - zero][~nan], other[~nan].to(torch.float8_e4m3fn).float())
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(17, 1, 64), (64, 2, 128), (71, 1, 48), (130, 1, 128), (256, 2, 16)])
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_groups_of_more_than_sixteen_heads(heads, kv_heads, dim, kind):
+    """A token alone then fills a tile of 64 or 128 rows, or several; in place, with a window, and with a few more tokens."""
+    lens = [1, 700, 33, 64, 0, 65, 2500]
+    c = filled(lens, 16, heads, kv_heads, dim, kind, heads)
+    q = (randn(gen(1), 7, heads, dim) * 1.5).bfloat16()
+    seqs, cu = ints([3, 1, -1, 0, 6, 4, 2]), ints(range(8))
+    want = check_attention(c, q, seqs, cu, max_q=1, max_len=2500)
+    check_attention(c, q, seqs, cu)
+    check_attention(c, q, seqs, cu, window=100, max_q=1)
+    got = q.clone()
+    c.attention(0, got, seqs, cu, max_q=1, max_len=2500, out=got)
+    assert torch.equal(torch.cat((got[:2], got[3:])), torch.cat((want[:2], want[3:]))) and torch.equal(got[2], q[2])
+    q = randn(gen(2), 12, heads, dim).bfloat16()
+    check_attention(c, q, ints([6, 1, 2]), ints([0, 5, 9, 12]), max_q=5)
+
+
+@pytest.mark.parametrize("page", [256, 512, 1024])
+@pytest.mark.parametrize("T", [1, 6, 40, 150])
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_large_pages(page, T, kind):
+    lens = [page - 1, page, page + 1, 2 * page + 77, T, 3 * page]
+    c = filled(lens, page, 14, 2, 64, kind, page + T)
+    q = randn(gen(5), 6 * T, 14, 64).bfloat16()
+    seqs, cu = ints([5, 0, 1, 4, 2, 3]), ints(range(0, 6 * T + 1, T))
+    check_attention(c, q, seqs, cu, max_q=T, max_len=3 * page)
+    check_attention(c, q, seqs, cu, window=page // 2, max_q=T)
+
+
+@pytest.mark.parametrize("kv_heads", [128, 300, 600])
+@pytest.mark.parametrize("T", [1, 20])
+def test_more_key_value_heads_than_workgroups_run_at_once(kv_heads, T):
+    """A long sequence is then cut in few chunks or none."""
+    c = filled([3000, 70], 32, kv_heads, kv_heads, 16, "bf16", kv_heads)
+    q = randn(gen(6), 2 * T, kv_heads, 16).bfloat16()
+    check_attention(c, q, ints([0, 1]), ints([0, T, 2 * T]), max_q=T)
