@@ -61,11 +61,9 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
         const float s = sc ? sc[h] : 1.f;
         const long page = slot >> a.lps;
         uint8_t* dst = (uint8_t*)(is_k ? a.k_pages : a.v_pages) + (((page * a.kv_heads + h) << a.lps) + (slot & ((1 << a.lps) - 1))) * a.hd + c;
+        const float by = s == 0.f ? 1.f : s, keep = s == 0.f ? 0.f : 1.f;      // a scale of 0 stores 0 (x / 0 would be 448 or no number); NaN stays NaN
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {                          // (a scale of 0 stores 0: x / 0 would be 448 or no number; NaN stays NaN)
-            y1[e] = s == 0.f ? clamp448(y1[e]) * 0.f : clamp448(y1[e] / s);
-            y2[e] = s == 0.f ? clamp448(y2[e]) * 0.f : clamp448(y2[e] / s);
-        }
+        for (int e = 0; e < 8; ++e) { y1[e] = clamp448(y1[e] / by) * keep; y2[e] = clamp448(y2[e] / by) * keep; }
         *(uint2*)dst = make_uint2(pack4_e4m3(y1[0], y1[1], y1[2], y1[3]), pack4_e4m3(y1[4], y1[5], y1[6], y1[7]));
         *(uint2*)(dst + half) = make_uint2(pack4_e4m3(y2[0], y2[1], y2[2], y2[3]), pack4_e4m3(y2[4], y2[5], y2[6], y2[7]));
     }
