@@ -3,7 +3,7 @@
 // The pair (x[d], x[d + D/2]) turns by the angle of its token's position (rows of the cos / sin table); the turn is done in fp32 on the bf16
 // inputs and rounded once, to bf16 or, for an 8-bit cache, x / scale clamped to +-448 to e4m3 (products of two bf16 values are exact in fp32,
 // so the sum is the only other rounding).  A thread owns eight pairs: 16-byte loads and stores, the table row comes from the L1.  Bound by the bytes:
-// 19,000 tokens of 28 / 4 heads of 128 (356 MB) 69 us, 5.1 TB/s (a large copy: 4.9); 16 tokens 3.4 us, a launch.
+// 19,000 tokens of 28 / 4 heads of 128 (356 MB) 69 us, 5.1 TB/s (a large copy: 4.9), into e4m3 pages (336 MB) 67; 16 tokens 3.4 us, a launch.
 #include "paged.h"
 
 static __device__ __forceinline__ unsigned pack4_e4m3(float a, float b, float c, float d) {

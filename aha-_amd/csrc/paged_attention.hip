@@ -479,8 +479,9 @@ __global__ __launch_bounds__(256) void paged_attn_rows_kernel(PagedAttnArgs a) {
 #endif
 // ---------------------------------------------------------------------------------------------
 // Many rows (frames, prompts): bound by the matrix cores and the exponentials.  A workgroup's four waves have 16 NT rows each and share blocks of
-// 64 keys, K and V double-buffered in LDS: the next block is under way while this one is computed, with one barrier a block.  bf16 pages go
-// straight to LDS (buffer_load ... lds, 1 KiB of contiguous rows an instruction), e4m3 through registers, where they become bf16.  In LDS a row's
+// 64 keys, K and V double-buffered in LDS, with one barrier a block.  bf16 pages go straight to LDS (buffer_load ... lds, 1 KiB of contiguous rows an
+// instruction), e4m3 through registers, where they become bf16.  The next block is under way during the first product and the softmax; bf16: the second
+// product begins with a wait for it, as the compiler cannot tell its transposing reads of V from the transfers into the other buffer.  In LDS a row's
 // 16-byte chunks are permuted by its number: sixteen rows read at one column, or eight rows at two, touch every bank once.
 // P is rounded to bf16 (half a step, 2^-8 of p, as the output itself is) unless the caller asks for two halves (HALVES: 2^-17); the sum of the row is
 // taken from the rounded values, by the matrix cores (a product with ones), so that numerator and denominator round alike.  One half / two, us: 8,192
@@ -869,7 +870,7 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a, i
         const long step = (long)a.kv_heads * TR, p0 = (slot * a.kv_heads + hk) * TR + (r - tile * TR);
         float M = -INFINITY, l = 0.f;
         f32x4 acc = {0.f, 0.f, 0.f, 0.f}, v[FLY];
-        const unsigned hop = (unsigned)step * (D * 4);      // (bytes: all partial results of a call are 34 MB at most)
+        const unsigned hop = (unsigned)step * (D * 4);      // (bytes: all partial results of a call are 67 MB at most: 1,024 x 128 rows of 512)
         const __amdgpu_buffer_rsrc_t po = __builtin_amdgcn_make_buffer_rsrc((void*)(a.part_o + p0 * D), 0, (unsigned)(chunks - 1) * hop + D * 4, 0x00020000);
         auto fetch = [&](int c) {                           // before their weights are known: those of chunks without keys are read and dropped
 #pragma unroll

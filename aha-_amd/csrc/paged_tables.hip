@@ -11,7 +11,7 @@
 // sequence -> length -> sum -> free entry -> store, each link a trip to the L2 or memory.  All requests are looked at before anything is
 // written, so a call that cannot be done (status) changes nothing.  Pages and tokens are dealt out flat, a thread finds the request of its
 // page or token by bisection of the sums in LDS: a request of two thousand tokens does not keep one thread busy.  16 requests of a token: reserve
-// 4.7 us, truncate 3.7; 256 of some 250 tokens (64,700): 7.7 and 4.0 for the slots, truncate 6.7.
+// 4.5 us, truncate 3.6; 256 of some 250 tokens (64,518): 7.6 and 4.5 for the slots, truncate 6.7.
 #include "paged.h"
 
 struct Scan2 { int a, b; };
