@@ -3,6 +3,8 @@ import pytest
 import torch
 
 import aha_amd  # noqa: F401
+from aha_amd.paged import PagedKVCache
+from aha_amd.runtime import AhaError
 from test_gpu_paged import DEV, check_attention, filled, gen, ints, pool, randn
 
 pytestmark = pytest.mark.gpu
@@ -82,3 +84,62 @@ def test_more_key_value_heads_than_workgroups_run_at_once(kv_heads, T):
     c = filled([3000, 70], 32, kv_heads, kv_heads, 16, "bf16", kv_heads)
     q = randn(gen(6), 2 * T, kv_heads, 16).bfloat16()
     check_attention(c, q, ints([0, 1]), ints([0, T, 2 * T]), max_q=T)
+
+
+@pytest.mark.parametrize("page", [16, 64, 128])
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_sequences_that_fill_their_tables(page, kind):
+    """No entry is left behind the last page, of the last sequence no table either; not one token more is reserved."""
+    lens = [5 * page, 3, 5 * page - 1, 5 * page]
+    c = filled(lens, page, 14, 2, 64, kind, page, spare=0)
+    c = PagedKVCache(c.n_pages, page, 2, 64, 4, 5, dtype=c.dtype, device=DEV, k_pages=c.k_pages, v_pages=c.v_pages, block_table=c.block_table[:, :5].contiguous(),
+                     lens=c.lens, k_scale=c.k_scale, v_scale=c.v_scale)
+    c.n_free.zero_()
+    for T in (1, 7, 40):
+        q = randn(gen(T), 4 * T, 14, 64).bfloat16()
+        check_attention(c, q, ints([3, 1, 2, 0]), ints(range(0, 4 * T + 1, T)), max_q=T)
+        check_attention(c, q, ints([3, 1, 2, 0]), ints(range(0, 4 * T + 1, T)), window=page + 5, max_q=T)
+    assert c.reserve(ints([2]), ints([1]), 1)[3].tolist() == [0, 0] and c.reserve(ints([2]), ints([1]), 1)[3].tolist() == [16, 0]
+    assert c.lens.tolist() == [5 * page, 3, 5 * page, 5 * page]
+
+
+@pytest.mark.parametrize("T,L", [(1, 300), (1, 3000), (6, 300), (40, 3000), (150, 300)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_a_query_that_is_no_number_stays_alone(T, L, bad):
+    c = filled([L, L - 70], 16, 14, 2, 64, "bf16", 51)
+    q = randn(gen(52), 2 * T, 14, 64).bfloat16()
+    seqs, cu = ints([0, 1]), ints([0, T, 2 * T])
+    want = c.attention(0, q, seqs, cu, max_q=T)
+    q[T // 2, 9, 5] = bad                                                    # times keys of both signs: no row of numbers either way
+    got = c.attention(0, q, seqs, cu, max_q=T)
+    assert bool(torch.isnan(got[T // 2, 9]).all())
+    got[T // 2, 9] = want[T // 2, 9]
+    assert torch.equal(got, want)
+
+
+def test_calls_from_two_threads():
+    """Each on a stream of its own over one pool; a refusal's message is its thread's."""
+    import threading
+    c = filled([900, 700], 16, 14, 2, 64, "bf16", 53)
+    qs = [randn(gen(54 + i), 2, 14, 64).bfloat16() for i in range(2)]
+    seqs, cu = ints([0, 1]), ints([0, 1, 2])
+    want, wrong = [c.attention(0, q, seqs, cu, max_q=1) for q in qs], []
+    torch.cuda.synchronize()
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = c.attention(0, qs[i], seqs, cu, max_q=1)
+                try:
+                    c.attention(0 if i else 7, qs[i], seqs, cu, scale=-1.0 if i else None)
+                except AhaError as e:
+                    wrong.extend([] if ("scale" if i else "layer") in str(e) else [str(e)])
+                torch.cuda.current_stream().synchronize()
+                wrong.extend([] if torch.equal(got, want[i]) else ["values"])
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong[:3]
