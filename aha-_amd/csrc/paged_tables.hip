@@ -48,6 +48,8 @@ static __device__ __forceinline__ int bisect(const int* end, int n, int x) {
 }
 
 #define PT_THREADS 1024
+// entries a thread keeps in registers from truncate's count to the list (256 requests of some 250 tokens: with a count and a list that both read them
+// 11.4 us, so 6.7)
 #define PT_KEEP 2
 struct Request { int seq, len, count, had, need, last, err; };     // had: pages it keeps; need: pages it takes (gives back); last: its page that is filled in part
 

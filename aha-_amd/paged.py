@@ -23,7 +23,8 @@ from . import lib as _l
 from .runtime import AhaError
 
 _ERRORS = ((1, "the free list is too short"), (2, "more new tokens than n_tokens"), (4, "a sequence out of range or a corrupt length"),
-           (8, "a sequence is listed twice"), (16, "a sequence outgrows its block table"), (32, "a negative count or a length out of range"), (64, "a new token's page, from the free list or the block table, is none"))
+           (8, "a sequence is listed twice"), (16, "a sequence outgrows its block table"), (32, "a negative count or a length out of range"),
+           (64, "a new token's page, from the free list or the block table, is none"))
 _TYPES = {torch.bfloat16: _l.KV_BF16, torch.float8_e4m3fn: _l.KV_E4M3}
 _MAX = 0x7fffffff
 
@@ -36,17 +37,16 @@ def _c_ints(*x):
 class PagedKVCache:
     """One pool.  `rope`: (cos, sin), bf16 [positions, head_dim], what `append` rotates with
     (positions behind its last as the last); without it keys and queries come rotated.
-    `k_scale` / `v_scale`: fp32 [layers, kv_heads] of an e4m3 pool (default 1), finite and not negative (0: that head's values are 0).  The tensors (`k_pages`, `v_pages`: [layers, n_pages, kv_heads,
-    page_size, head_dim]; `block_table` [max_seqs, max_blocks], `lens` [max_seqs], `free_pages` [n_pages], `n_free` [1], all int32) are made
-    here unless given, and are the caller's to look at; pages may hold anything.  `precise`: the attention of drafts, frames and prompts keeps its
+    `k_scale` / `v_scale`: fp32 [layers, kv_heads] of an e4m3 pool (default 1), finite and not negative (0: that head's values are 0).
+    The tensors (`k_pages`, `v_pages`: [layers, n_pages, kv_heads, page_size, head_dim]; `block_table` [max_seqs, max_blocks],
+    `lens` [max_seqs], `free_pages` [n_pages], `n_free` [1], all int32) are made here unless given, and are the caller's to look at; pages may hold anything.  `precise`: the attention of drafts, frames and prompts keeps its
     probabilities to 2^-17 (a token's always are) instead of rounding them to bf16, as the ring caches' attention does; up to half as slow again."""
 
     def __init__(self, n_pages: int, page_size: int, kv_heads: int, head_dim: int, max_seqs: int, max_blocks: int, *, layers: int = 1,
                  dtype: torch.dtype = torch.bfloat16, device="cuda:0", rope: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
                  k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None, k_pages: Optional[torch.Tensor] = None,
                  v_pages: Optional[torch.Tensor] = None, block_table: Optional[torch.Tensor] = None, lens: Optional[torch.Tensor] = None,
-                 free_pages: Optional[torch.Tensor] = None, n_free: Optional[torch.Tensor] = None,
-                 precise: bool = False):
+                 free_pages: Optional[torch.Tensor] = None, n_free: Optional[torch.Tensor] = None, precise: bool = False):
         self.handle = None
         self.lib = _l.get()
         dev = torch.device(device)
